@@ -23,6 +23,7 @@
  *                          and its backward straight into the parameter grads
  *   sv2n_head_*            GATModel's final Linear (a4) fwd/bwd
  *   sv2n_adam_f32          the reference's Adam step over flat buffers (a13)
+ *   sv2n_layer_norm_*      layer norm between the GAT layers, fwd / bwd
  *   sv2n_gat_attn_tiled_*  the same attention fwd/bwd for 32 < n <= 256 (C5
  *                          stress shapes), target-row-tiled
  *   sv2n_gat_attn_fused_*  32 < n <= 256 with narrow edge features: the edge
@@ -76,8 +77,14 @@ extern "C" {
 #define SV2N_MAX_N_TILED 256 /* nodes per graph on the tiled attention path
                                (sv2n_gat_attn_tiled_*) and the edge pass   */
 #define SV2N_MAX_HEADS 8    /* attention heads per layer                   */
+#define SV2N_LN_MAX_COLS 16384 /* widest layer-norm row                     */
 #define SV2N_TICKET_WORDS 288 /* counter words of a two-level in-launch ticket
                                  (Adam counter, head workspace header)     */
+
+/* element types of the entries that take more than one */
+#define SV2N_DT_F32  0
+#define SV2N_DT_BF16 1
+#define SV2N_DT_F16  2
 
 /* argument errors (negative return codes) */
 #define SV2N_ERR_ARG       (-1)  /* null pointer / non-positive size        */
@@ -697,6 +704,29 @@ int sv2n_window_gather_cv(const float* vol, const float* volvol, const float* di
                           int64_t num_windows, int seq_length, int future_steps,
                           const uint16_t* canon, float* x, uint16_t* x_bf16, int64_t ld_xb,
                           float* edge_attr, float* y, hipStream_t stream);
+
+/* Layer norm over rows of `cols` elements: z = (x - mean)·rstd with rstd =
+ * 1/sqrt(var + eps) (biased variance), y = z·weight + bias.
+ *   x       [rows][ldx >= cols] of `dtype` (SV2N_DT_*), any alignment of that
+ *           type; y [rows][cols] dense, the same type.
+ *   weight, bias  [cols] of `wdtype` (SV2N_DT_F32, or the rows' type); either
+ *           may be NULL (1 and 0).
+ *   mean, rstd  [rows] f32, what the backward needs; may be NULL.
+ * Sums and statistics are f32 whatever the type.  cols <= SV2N_LN_MAX_COLS;
+ * rows may be 0. */
+int sv2n_layer_norm_fwd(const void* x, int64_t ldx, int dtype, const void* weight,
+                        const void* bias, int wdtype, int64_t rows, int cols, float eps, void* y,
+                        float* mean, float* rstd, hipStream_t stream);
+/* Its backward, with the forward's mean and rstd: dx [rows][cols] dense, dw and
+ * db [cols] of `wdtype`; each may be NULL (not computed).  accumulate != 0: dw
+ * and db are added to instead of overwritten.  dw and db are summed in a fixed
+ * order (the same bits every run).  workspace (needed for dw / db):
+ * sv2n_layer_norm_bwd_workspace floats, scratch of this call alone. */
+int64_t sv2n_layer_norm_bwd_workspace(int64_t rows, int cols, int dtype);
+int sv2n_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, int dtype,
+                        const void* weight, int wdtype, const float* mean, const float* rstd,
+                        int64_t rows, int cols, void* dx, void* dw, void* db, int accumulate,
+                        float* workspace, int64_t workspace_floats, hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -125,6 +125,13 @@ _SIGNATURES = {
     "sv2n_adam_f32": (_i32, [_p, _p, _p, _p, _i64, _p, _f32, _f32, _f32, _f32, _f32, _p]),
     "sv2n_adam_f32_step": (_i32, [_p, _p, _p, _p, _i64, _p, _p, _f32, _f32, _f32, _f32, _f32,
                                   _p]),
+    # x ldx dtype weight bias wdtype rows cols eps y mean rstd stream
+    "sv2n_layer_norm_fwd": (_i32, [_p, _i64, _i32, _p, _p, _i32, _i64, _i32, _f32, _p, _p, _p,
+                                   _p]),
+    "sv2n_layer_norm_bwd_workspace": (_i64, [_i64, _i32, _i32]),
+    # dy lddy x ldx dtype weight wdtype mean rstd rows cols dx dw db accumulate ws ws_n stream
+    "sv2n_layer_norm_bwd": (_i32, [_p, _i64, _p, _i64, _i32, _p, _i32, _p, _p, _i64, _i32, _p,
+                                   _p, _p, _i32, _p, _i64, _p]),
     "sv2n_dropout_uniform": (_i32, [_p, _i64, _u64, _p, _u32, _p]),
     "sv2n_edge_logits_fwd_cv": (_i32, [_p, _i64, _i32, _i32, _p, _p, _i32, _p, _i32, _i32, _p]),
     "sv2n_edge_logits_bwd_cv_workspace": (_i64, [_i32, _i32]),
