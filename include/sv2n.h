@@ -23,6 +23,8 @@
  *                          and its backward straight into the parameter grads
  *   sv2n_head_*            GATModel's final Linear (a4) fwd/bwd
  *   sv2n_adam_f32          the reference's Adam step over flat buffers (a13)
+ *   sv2n_orthogonalize     Newton-Schulz orthogonalisation of a matrix, and
+ *   sv2n_muon_step         the optimiser step over weight matrices built on it
  *   sv2n_layer_norm_*      layer norm between the GAT layers, fwd / bwd
  *   sv2n_gat_attn_tiled_*  the same attention fwd/bwd for 32 < n <= 256 (C5
  *                          stress shapes), target-row-tiled
@@ -78,6 +80,9 @@ extern "C" {
                                (sv2n_gat_attn_tiled_*) and the edge pass   */
 #define SV2N_MAX_HEADS 8    /* attention heads per layer                   */
 #define SV2N_LN_MAX_COLS 16384 /* widest layer-norm row                     */
+#define SV2N_NS_MAX_SIDE 16384 /* largest side of an orthogonalised matrix  */
+#define SV2N_NS_MAX_BATCH 1024 /* matrices of one orthogonalised stack      */
+#define SV2N_NS_MAX_STEPS 32
 #define SV2N_TICKET_WORDS 288 /* counter words of a two-level in-launch ticket
                                  (Adam counter, head workspace header)     */
 
@@ -727,6 +732,42 @@ int sv2n_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx
                         const void* weight, int wdtype, const float* mean, const float* rstd,
                         int64_t rows, int cols, void* dx, void* dw, void* db, int accumulate,
                         float* workspace, int64_t workspace_floats, hipStream_t stream);
+
+/* Newton-Schulz orthogonalisation: X = G / max(|G|_F, eps), then `steps` times
+ * S = X Xt, X <- a X + (b S + c S S) X, on the transpose where G has more rows
+ * than columns; the result has G's shape and its singular values near 1.
+ *   g    [batch][rows][ld >= cols] of `dtype` (SV2N_DT_*), matrices
+ *        batch_stride elements apart; each is normalised on its own.
+ *   out  [batch][rows][cols] dense, of `dtype`; must not overlap g.
+ * f32-accurate products whatever the type; the result is rounded once.
+ * Sides up to SV2N_NS_MAX_SIDE, steps 1..SV2N_NS_MAX_STEPS, batch up to
+ * SV2N_NS_MAX_BATCH.  Coefficients that let a singular value grow past 256 are
+ * refused.  workspace: sv2n_orthogonalize_workspace bytes, 256-B aligned,
+ * scratch of this call alone. */
+int64_t sv2n_orthogonalize_workspace(int64_t batch, int64_t rows, int64_t cols);
+int sv2n_orthogonalize(const void* g, int64_t ld, int64_t batch_stride, int dtype, int64_t batch,
+                       int64_t rows, int64_t cols, int steps, float a, float b, float c, float eps,
+                       void* out, void* workspace, int64_t workspace_bytes, hipStream_t stream);
+
+/* One optimiser step over `count` weight matrices (host array), f32 and dense:
+ *   momentum <- beta·momentum + (1 - beta)·grad
+ *   U = orthogonalised ((1 - beta)·grad + beta·momentum), or of the momentum
+ *       itself without nesterov
+ *   weight <- (1 - lr·weight_decay)·weight - lr·lr_scale·U
+ * No buffer of one matrix may overlap a weight or momentum of another, or one of
+ * its own (the caller's duty).  workspace: sv2n_muon_step_workspace bytes,
+ * 256-B aligned, scratch of this call alone. */
+typedef struct sv2n_muon_matrix {
+  float* weight;
+  const float* grad;
+  float* momentum;
+  int rows, cols;
+  float lr_scale;
+} sv2n_muon_matrix;
+int64_t sv2n_muon_step_workspace(const sv2n_muon_matrix* mats, int count);
+int sv2n_muon_step(const sv2n_muon_matrix* mats, int count, double lr, double momentum,
+                   int nesterov, double weight_decay, int steps, float a, float b, float c, float eps,
+                   void* workspace, int64_t workspace_bytes, hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -10,6 +10,7 @@ from .data import Batch, Data, WindowDataset, collate, shard_indices, synthetic_
     synthetic_series, window_batch, window_graph
 from .layout import GraphLayout, UnsupportedLayout, analyze_edge_index, canonical_edge_index
 from .model import GATModel
+from .muon import Muon, muon_step, orthogonalize
 from .norm import LayerNorm, layer_norm
 from . import evaluate, series
 
@@ -17,4 +18,5 @@ __all__ = [
     "GATConv", "GATModel", "Linear", "Data", "Batch", "collate", "window_graph", "window_batch",
     "synthetic_batch", "synthetic_series", "WindowDataset", "GraphLayout", "UnsupportedLayout",
     "analyze_edge_index", "canonical_edge_index", "shard_indices", "LayerNorm", "layer_norm",
+    "Muon", "muon_step", "orthogonalize",
 ]

@@ -23,6 +23,7 @@ _p = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 _u32 = ctypes.c_uint32
 _u64 = ctypes.c_uint64
 
@@ -44,6 +45,12 @@ class EdgeGradLayer(ctypes.Structure):
         ("W_edge", _p), ("att_edge", _p), ("gW_edge", _p), ("g_att_edge", _p),
         ("heads", _i32), ("channels", _i32), ("col0", _i32),
     ]
+
+
+class MuonMatrix(ctypes.Structure):
+    """sv2n_muon_matrix (include/sv2n.h)."""
+    _fields_ = [("weight", _p), ("grad", _p), ("momentum", _p), ("rows", _i32), ("cols", _i32),
+                ("lr_scale", _f32)]
 
 
 # name -> (restype, argtypes); mirrors include/sv2n.h
@@ -132,6 +139,14 @@ _SIGNATURES = {
     # dy lddy x ldx dtype weight wdtype mean rstd rows cols dx dw db accumulate ws ws_n stream
     "sv2n_layer_norm_bwd": (_i32, [_p, _i64, _p, _i64, _i32, _p, _i32, _p, _p, _i64, _i32, _p,
                                    _p, _p, _i32, _p, _i64, _p]),
+    "sv2n_orthogonalize_workspace": (_i64, [_i64, _i64, _i64]),
+    # g ld batch_stride dtype batch rows cols steps a b c eps out ws ws_bytes stream
+    "sv2n_orthogonalize": (_i32, [_p, _i64, _i64, _i32, _i64, _i64, _i64, _i32, _f32, _f32, _f32,
+                                  _f32, _p, _p, _i64, _p]),
+    "sv2n_muon_step_workspace": (_i64, [_p, _i32]),
+    # mats count lr momentum nesterov weight_decay steps a b c eps ws ws_bytes stream
+    "sv2n_muon_step": (_i32, [_p, _i32, _f64, _f64, _i32, _f64, _i32, _f32, _f32, _f32, _f32, _p,
+                              _i64, _p]),
     "sv2n_dropout_uniform": (_i32, [_p, _i64, _u64, _p, _u32, _p]),
     "sv2n_edge_logits_fwd_cv": (_i32, [_p, _i64, _i32, _i32, _p, _p, _i32, _p, _i32, _i32, _p]),
     "sv2n_edge_logits_bwd_cv_workspace": (_i64, [_i32, _i32]),

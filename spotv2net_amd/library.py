@@ -124,6 +124,10 @@ _SCHEMAS = {
                       "-> (Tensor, Tensor, Tensor)",
     "layer_norm_bwd_acc": "(Tensor dy, Tensor x, Tensor? weight, Tensor mean, Tensor rstd, "
                           "Tensor(a!)? g_weight, Tensor(b!)? g_bias) -> Tensor",
+    "orthogonalize": "(Tensor g, int steps, float a, float b, float c, float eps) -> Tensor",
+    "muon_step": "(Tensor(a!)[] weights, Tensor[] grads, Tensor(b!)[] momenta, float[] lr_scales, "
+                 "float lr, float momentum, bool nesterov, float weight_decay, int steps, float a, "
+                 "float b, float c, float eps) -> ()",
     "window_gather": "(Tensor vol, Tensor volvol, Tensor starts, int seq_length, "
                      "int future_steps, Tensor canon, Tensor(a!) x, Tensor(b!) edge_attr, "
                      "Tensor(c!) y, int start_offset=0, Tensor? diag=None, "
@@ -1421,3 +1425,112 @@ def _layer_norm_bwd_acc(dy, x, weight, mean, rstd, g_weight, g_bias):
 @_fake("layer_norm_bwd_acc")
 def _layer_norm_bwd_acc_fake(dy, x, weight, mean, rstd, g_weight, g_bias):
     return torch.empty(x.shape, device=x.device, dtype=x.dtype)
+
+
+# --------------------------------------------------------------------------
+# Newton-Schulz orthogonalisation and the optimiser step built on it
+# (sv2n_orthogonalize, sv2n_muon_step)
+# --------------------------------------------------------------------------
+NS_MAX_SIDE, NS_MAX_BATCH, NS_MAX_STEPS = 16384, 1024, 32  # SV2N_NS_MAX_*
+
+
+def _ns_check(steps, eps) -> None:
+    _need(1 <= steps <= NS_MAX_STEPS, f"orthogonalize: 1 to {NS_MAX_STEPS} steps, got {steps}")
+    _need(eps > 0.0, f"orthogonalize: eps must be positive, got {eps}")
+
+
+def _ns_rc(rc: int, what: str) -> None:
+    _need(rc != -1, f"{what}: coefficients that are not finite, or let singular values grow past 256")
+    _lib.check(rc, what)
+
+
+@_impl("orthogonalize")
+def _orthogonalize(g, steps, a, b, c, eps):
+    _need(g.dtype in _DT, f"orthogonalize: expected float32, bfloat16 or float16, got {g.dtype}")
+    _need(g.dim() in (2, 3), f"orthogonalize: expected a matrix or a stack of them, got {g.dim()}-D")
+    _ns_check(steps, eps)
+    rows, cols = g.shape[-2:]
+    batch = g.shape[0] if g.dim() == 3 else 1
+    _need(rows <= NS_MAX_SIDE and cols <= NS_MAX_SIDE and batch <= NS_MAX_BATCH,
+          f"orthogonalize: sides up to {NS_MAX_SIDE}, up to {NS_MAX_BATCH} matrices, got "
+          f"{tuple(g.shape)}")
+    out = torch.empty(g.shape, device=g.device, dtype=g.dtype)
+    if out.numel() == 0:
+        return out
+    if (cols > 1 and g.stride(-1) != 1) or (rows > 1 and g.stride(-2) < cols):
+        g = g.contiguous()
+    lib = _lib.load()
+    n = lib.sv2n_orthogonalize_workspace(batch, rows, cols)
+    ws = torch.empty(n, device=g.device, dtype=torch.uint8)
+    with _on_device(g):
+        _ns_rc(lib.sv2n_orthogonalize(
+            g.data_ptr(), g.stride(-2) if rows > 1 else cols, g.stride(0) if batch > 1 else 0,
+            _DT[g.dtype], batch, rows, cols, steps, a, b, c, eps, out.data_ptr(), ws.data_ptr(), n,
+            _st(g)), "sv2n_orthogonalize")
+    return out
+
+
+@_fake("orthogonalize")
+def _orthogonalize_fake(g, steps, a, b, c, eps):
+    return torch.empty(g.shape, device=g.device, dtype=g.dtype)
+
+
+def _muon_disjoint(mats) -> bool:
+    """Whether no weight or momentum shares memory with any other buffer of the
+    step (gradients, which are only read, may share among themselves)."""
+    spans = []
+    for w, g, m in mats:
+        for t, written in ((w, True), (g, False), (m, True)):
+            spans.append((t.data_ptr(), t.data_ptr() + 4 * t.numel(), written))
+    spans.sort()
+    end_any = end_written = 0
+    for lo, hi, written in spans:
+        if lo < end_written or (written and lo < end_any):
+            return False
+        end_any = max(end_any, hi)
+        if written:
+            end_written = max(end_written, hi)
+    return True
+
+
+@_impl("muon_step")
+def _muon_step(weights, grads, momenta, lr_scales, lr, momentum, nesterov, weight_decay, steps, a,
+               b, c, eps):
+    k = len(weights)
+    _need(len(grads) == len(momenta) == len(lr_scales) == k, "muon_step: lists of different lengths")
+    _ns_check(steps, eps)
+    _need(0.0 <= momentum < 1.0, f"muon_step: momentum must be in [0, 1), got {momentum}")
+    mats, scales = [], []
+    for w, g, m, s in zip(weights, grads, momenta, lr_scales):
+        _f32(w, g, m)
+        _need(w.dim() == 2, f"muon_step: weights are matrices, got shape {tuple(w.shape)}")
+        _need(g.shape == w.shape == m.shape, f"muon_step: weight {tuple(w.shape)}, gradient "
+              f"{tuple(g.shape)}, momentum {tuple(m.shape)}")
+        _need(w.device == g.device == m.device == weights[0].device,
+              "muon_step: buffers on different devices")
+        _need(max(w.shape) <= NS_MAX_SIDE, f"muon_step: sides up to {NS_MAX_SIDE}, got "
+              f"{tuple(w.shape)}")
+        _dense(w, m)
+        if w.numel():
+            mats.append((w, g.contiguous(), m))
+            scales.append(s)
+    if not mats:
+        return
+    _need(_muon_disjoint(mats), "muon_step: a weight or momentum shares memory with another buffer")
+    arr = (_lib.MuonMatrix * len(mats))()
+    for i, ((w, g, m), s) in enumerate(zip(mats, scales)):
+        arr[i] = _lib.MuonMatrix(w.data_ptr(), g.data_ptr(), m.data_ptr(), w.shape[0], w.shape[1], s)
+    lib = _lib.load()
+    p = ctypes.addressof(arr)
+    n = lib.sv2n_muon_step_workspace(p, len(mats))
+    w0 = mats[0][0]
+    ws = torch.empty(n, device=w0.device, dtype=torch.uint8)
+    with _on_device(w0):
+        _ns_rc(lib.sv2n_muon_step(p, len(mats), lr, momentum, int(nesterov), weight_decay, steps, a,
+                                  b, c, eps, ws.data_ptr(), n, _st(w0)), "sv2n_muon_step")
+
+
+@_fake("muon_step")
+def _muon_step_fake(weights, grads, momenta, lr_scales, lr, momentum, nesterov, weight_decay, steps,
+                    a, b, c, eps):
+    return None
