@@ -19,8 +19,14 @@
 // (X for S, Xt for Q X), so one kernel with one staging scheme serves all three
 // products; the epilogue writes X and Xt of the next step.
 //
-// Layout of an operand: [row][K/32][plane hi, lo][32 halves], rows and K padded
-// with zeros to the tile: the 32 K values a stage needs of a row are one 128-B line.
+// Layout of an operand: MFMA fragments in order.  A block of 32 rows x 16 K values
+// is 64 lanes x 8 halves (1 KiB) as v_mfma_f32_32x32x16_f16 reads it, hi plane then
+// lo, blocks along K next to each other, rows and K padded with zeros: a wave's
+// fragment is one contiguous KiB, from memory or LDS alike (no bank conflicts, no
+// swizzle).  Inside the 16 K values lane half h holds k = 4h..4h+3 and 8+4h..8+4h+3
+// (every operand agrees, so the sums do not care): that is how the accumulators
+// hold a tile's rows, so the tile's transpose goes back to memory as the next
+// product's fragments straight from registers.
 //
 // Several matrices (a model's weights) share each launch: `first` maps blocks to
 // matrices, so a step over four weights costs the same 3·steps + 2 launches as one.
@@ -31,12 +37,11 @@
 namespace sv2n {
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int NS_MAX = 16;      // matrices of one launch
-constexpr int NS_PARTS = 512;   // most partial sums of squares of one matrix
-constexpr int NS_PART_ELEMS = 8192;
+constexpr int NS_PARTS = 1024;  // most partial sums of squares of one matrix
+constexpr int NS_PART_ELEMS = 4096;
 
 struct NsMat {
   const void* g;        // [batch][rows][ld] of dtype
@@ -47,7 +52,7 @@ struct NsMat {
   int m, n, mp, np;     // m <= n, padded to the tile
   int batch, flip;      // flip: X = Gt
   int dtype;
-  int parts, part_rows; // partial sums of squares per matrix, rows of each
+  int parts, part_elems; // partial sums of squares per matrix, elements of each
   float lr;             // the update's factor (with buf)
   _Float16 *x, *xt[2], *s, *q;
   double* part;         // [batch][parts]
@@ -72,16 +77,13 @@ __device__ __forceinline__ int ns_find(const NsArgs& A, int b) {
   return i;
 }
 
-__device__ __forceinline__ float ns_ld(const void* p, int64_t i, int dtype) {
-  if (dtype == SV2N_DT_F32) return ((const float*)p)[i];
-  if (dtype == SV2N_DT_BF16) return (float)((const __bf16*)p)[i];
-  return (float)((const _Float16*)p)[i];
+// halves from an operand's start to the hi fragment block of rows 32·r32.., K values
+// 16·k16.. of depth kp; the lo block follows it
+__device__ __forceinline__ int64_t ns_blk(int64_t r32, int k16, int kp) {
+  return (r32 * (kp >> 4) + k16) << 10;
 }
-
-// halves offset of (row, k) of the hi plane in an operand of padded depth kp; lo: + 32
-__device__ __forceinline__ int64_t ns_off(int64_t row, int k, int kp) {
-  return row * (2 * (int64_t)kp) + ((k >> 5) << 6) + (k & 31);
-}
+// the 16 K values of a block that lane half h holds, in register order
+__device__ __forceinline__ int ns_k(int h, int e) { return ((e & 4) << 1) + 4 * h + (e & 3); }
 
 // the matrix the products orthogonalise: G, or its momentum update
 __device__ __forceinline__ float ns_update(const NsScale& sc, float g, float buf) {
@@ -90,32 +92,54 @@ __device__ __forceinline__ float ns_update(const NsScale& sc, float g, float buf
 
 // ---- 1: the momentum and the partial sums of squares (in 64 bits: an f32 square
 // overflows above 2^64 and is lost below 2^-75) ----
+// A block takes part_elems elements of a matrix, 16 B a thread and load where the rows
+// are dense and aligned, else one by one.
+template <typename T>
 __global__ __launch_bounds__(256) void k_ns_norm(NsArgs A, NsScale sc) {
+  constexpr int V = 16 / (int)sizeof(T);
   __shared__ double red[4];
   const int mi = ns_find(A, blockIdx.x);
   const NsMat& M = A.mat[mi];
   const int local = blockIdx.x - A.first[mi];
   const int b = local / M.parts, p = local - b * M.parts;
-  // tx threads along a row, the rest down the rows
-  int tx = 256;
-  while (tx > 1 && tx / 2 >= M.cols) tx >>= 1;
-  const int ty = 256 / tx;
-  const int c0 = threadIdx.x % tx, r0 = threadIdx.x / tx;
-  const int64_t rbeg = (int64_t)p * M.part_rows;
-  const int64_t rend = min((int64_t)M.rows, rbeg + M.part_rows);
-  const int64_t base = b * M.g_batch;
+  const int total = M.rows * M.cols;
+  const int beg = p * M.part_elems, end = min(total, beg + M.part_elems);
+  const T* g = (const T*)M.g + b * M.g_batch;
+  float* buf = M.buf;
   double acc = 0.0;
-  for (int64_t r = rbeg + r0; r < rend; r += ty) {
-    for (int c = c0; c < M.cols; c += tx) {
-      float v = ns_ld(M.g, base + r * M.ld + c, M.dtype);
-      if (M.buf) {
-        float* bp = M.buf + r * M.cols + c;
-        const float nb = fmaf(sc.momentum, *bp, sc.fresh * v);
-        *bp = nb;
-        v = ns_update(sc, v, nb);
-      }
-      acc = fma((double)v, (double)v, acc);
+  auto take = [&](float v, float* bp) {
+    if (bp) {
+      const float nb = fmaf(sc.momentum, *bp, sc.fresh * v);
+      *bp = nb;
+      v = ns_update(sc, v, nb);
     }
+    acc = fma((double)v, (double)v, acc);
+  };
+  const bool vec = M.ld == M.cols && (((uintptr_t)g | (uintptr_t)buf) & 15) == 0;
+  int e = beg;
+  if (vec) {
+    // (beg is a multiple of 8)
+#pragma unroll 4
+    for (int i = beg + (int)threadIdx.x * V; i + V <= end; i += 256 * V) {
+      T t[V];
+      __builtin_memcpy(t, __builtin_assume_aligned(g + i, 16), 16);
+      float bv[V];
+      if (buf) {
+        __builtin_memcpy(bv, __builtin_assume_aligned(buf + i, 16), sizeof(bv));
+#pragma unroll
+        for (int j = 0; j < V; ++j) take((float)t[j], &bv[j]);
+        __builtin_memcpy(__builtin_assume_aligned(buf + i, 16), bv, sizeof(bv));
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) take((float)t[j], nullptr);
+      }
+    }
+    e = beg + (end - beg) / V * V;
+  }
+#pragma unroll 4
+  for (int i = e + (int)threadIdx.x; i < end; i += 256) {
+    const int r = i / M.cols, c = i - r * M.cols;
+    take((float)g[r * M.ld + c], buf ? buf + i : nullptr);
   }
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) acc += __shfl_xor(acc, o, 64);
@@ -130,6 +154,7 @@ __device__ __forceinline__ void ns_split(float v, _Float16& hi, _Float16& lo) {
 }
 
 // ---- 2: X_0 and its transpose as planes, one 64 x 64 tile per block ----
+template <typename T>
 __global__ __launch_bounds__(256) void k_ns_split(NsArgs A, NsScale sc) {
   __shared__ float tile[64][65];
   __shared__ double red[4];
@@ -140,6 +165,26 @@ __global__ __launch_bounds__(256) void k_ns_split(NsArgs A, NsScale sc) {
   const int b = local / (ti * tj);
   local -= b * ti * tj;
   const int i0 = (local / tj) * 64, j0 = (local % tj) * 64;
+  // the tile's elements first: their loads are in flight while the norm is added up
+  const T* g = (const T*)M.g + b * M.g_batch;
+  const int r0 = M.flip ? j0 : i0, c0 = M.flip ? i0 : j0;
+  const int c = threadIdx.x & 63, rq = threadIdx.x >> 6;
+  float v[16];
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    const int r = r0 + rq + 4 * k;
+    v[k] = r < M.rows && c0 + c < M.cols ? (float)g[(int64_t)r * M.ld + c0 + c] : 0.f;
+  }
+  if (M.buf) {
+    float m[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const int r = r0 + rq + 4 * k;
+      m[k] = r < M.rows && c0 + c < M.cols ? M.buf[(int64_t)r * M.cols + c0 + c] : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < 16; ++k) v[k] = ns_update(sc, v[k], m[k]);
+  }
   // every block adds the matrix's partials in the same order
   double acc = 0.0;
   for (int k = threadIdx.x; k < M.parts; k += 256) acc += M.part[(int64_t)b * M.parts + k];
@@ -151,40 +196,35 @@ __global__ __launch_bounds__(256) void k_ns_split(NsArgs A, NsScale sc) {
   // NaN stays NaN (fmax would drop it)
   const double den = norm < (double)sc.eps ? (double)sc.eps : norm;
   const double inv = ldexp(1.0, sc.kx) / den;
-  const int64_t base = b * M.g_batch;
-  const int r0 = M.flip ? j0 : i0, c0 = M.flip ? i0 : j0;
-  const int c = threadIdx.x & 63;
-#pragma unroll 4
+#pragma unroll
   for (int k = 0; k < 16; ++k) {
-    const int r = (threadIdx.x >> 6) + 4 * k;
-    float v = 0.f;
-    if (r0 + r < M.rows && c0 + c < M.cols) {
-      v = ns_ld(M.g, base + (int64_t)(r0 + r) * M.ld + c0 + c, M.dtype);
-      if (M.buf) v = ns_update(sc, v, M.buf[(int64_t)(r0 + r) * M.cols + c0 + c]);
-      v = (float)((double)v * inv);
-    }
-    if (M.flip) tile[c][r] = v; else tile[r][c] = v;
+    const int r = rq + 4 * k;
+    const float x = (float)((double)v[k] * inv);
+    if (M.flip) tile[c][r] = x; else tile[r][c] = x;
   }
   __syncthreads();
   _Float16* X = M.x + (int64_t)b * 2 * M.mp * M.np;
   _Float16* XT = M.xt[0] + (int64_t)b * 2 * M.mp * M.np;
+  // 8 fragment blocks of X (2 row groups x 4), then 8 of its transpose
+  const int lane = threadIdx.x & 63;
 #pragma unroll
-  for (int h = 0; h < 4; ++h) {
-    const int u = h * 256 + threadIdx.x;       // 512 groups of 8 values, then the transpose's
-    const int row = (u >> 3) & 63, k0 = (u & 7) * 8;
+  for (int u = threadIdx.x >> 6; u < 16; u += 4) {
+    const bool tr = u >= 8;
+    const int rg = (u >> 2) & 1, kg = u & 3;
+    const int row = rg * 32 + (lane & 31);
     f16x8 hi, lo;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float v = u < 512 ? tile[row][k0 + e] : tile[k0 + e][row];
-      _Float16 a, d;
-      ns_split(v, a, d);
-      hi[e] = a;
-      lo[e] = d;
+      const int k = kg * 16 + ns_k(lane >> 5, e);
+      _Float16 h, l;
+      ns_split(tr ? tile[k][row] : tile[row][k], h, l);
+      hi[e] = h;
+      lo[e] = l;
     }
-    _Float16* o = u < 512 ? X + ns_off(i0 + row, j0 + k0, M.np)
-                          : XT + ns_off(j0 + row, i0 + k0, M.mp);
-    *(f16x8*)o = hi;
-    *(f16x8*)(o + 32) = lo;
+    _Float16* o = tr ? XT + ns_blk(j0 / 32 + rg, i0 / 16 + kg, M.mp)
+                     : X + ns_blk(i0 / 32 + rg, j0 / 16 + kg, M.np);
+    *(f16x8*)(o + lane * 8) = hi;
+    *(f16x8*)(o + 512 + lane * 8) = lo;
   }
 }
 
@@ -197,99 +237,304 @@ __device__ __forceinline__ void ns_wave_sync() {
 
 enum { NS_S = 0, NS_Q = 1, NS_X = 2, NS_LAST = 3 };
 
-// Stores a wave's 32 x 32 tile of values (LDS, stride 33) as planes with row r0
-// and column (K) c0: two lanes per row, 128 B of hi and lo each.  TR: the tile's
-// transpose.
-template <bool TR>
-__device__ __forceinline__ void ns_store(const float* t, _Float16* dst, int64_t r0, int c0, int kp) {
-  const int lane = threadIdx.x & 63;
-  const int row = lane >> 1, k0 = (lane & 1) * 16;
-  _Float16* o = dst + ns_off(r0 + row, c0 + k0, kp);
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    f16x8 hi, lo;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int k = k0 + h * 8 + e;
-      _Float16 a, d;
-      ns_split(TR ? t[k * 33 + row] : t[row * 33 + k], a, d);
-      hi[e] = a;
-      lo[e] = d;
-    }
-    *(f16x8*)(o + h * 8) = hi;
-    *(f16x8*)(o + h * 8 + 32) = lo;
-  }
-}
-
-// ---- 3: one product ----
-// D[i][j] = sum_k P[i][k] R[j][k] over TB x TB tiles, 4 waves in a 2 x 2 grid of
-// TB/2 x TB/2.  A stage is 32 K values of both planes (128 B a row), staged
-// through registers into one of two LDS buffers: the next stage's loads are in
-// flight while this one is multiplied, one barrier a stage.  16-B slots of a row
-// are swapped by (row >> 1) & 7 so that the 16 rows a quarter wave reads fall on
-// different banks.
+// What a product computes; D = P Rt, 32 x 32 tiles [i][j]
 //   NS_S:  P = R = X,        S = D             (i >= j tiles, stored twice)
 //   NS_Q:  P = R = S,        Q = b S + c D     (the same)
 //   NS_X:  P = Q, R = Xt,    X' = a X + D      (X' and its transpose)
 //   NS_LAST: as NS_X, the result goes to the caller
+struct NsOut {
+  float up, old;        // new value = up·D + old·(the old S or X there)
+  float down;           // NS_LAST: to the caller's scale
+};
+template <int EPI>
+__device__ __forceinline__ NsOut ns_out(const NsScale& sc, const NsMat& M) {
+  NsOut o;
+  o.old = 0.f;
+  o.down = 0.f;
+  if (EPI == NS_S) {
+    o.up = ldexpf(1.f, sc.ks - 2 * sc.kx);
+  } else if (EPI == NS_Q) {
+    o.up = sc.c * ldexpf(1.f, sc.kq - 2 * sc.ks);
+    o.old = sc.b * ldexpf(1.f, sc.kq - sc.ks);
+  } else {
+    o.up = ldexpf(1.f, -sc.kq);
+    o.old = sc.a;
+    o.down = ldexpf(1.f, -sc.kx) * (M.buf ? -M.lr : 1.f);
+  }
+  return o;
+}
+
+// One 32 x 32 tile of D (accumulator layout: lane & 31 the column j, and rows
+// i = 8·(e/4) + 4·(lane/32) + e%4) at rows ib, columns jb: the new values, stored
+// where the next product reads them.  `tile`: 32 x 33 floats of the wave's own LDS,
+// for the orientation that registers do not give.
+template <int EPI>
+__device__ __forceinline__ void ns_epilogue(const f32x16& d, const NsOut& o, const NsMat& M,
+                                            const NsScale& sc, const _Float16* R, int64_t bt,
+                                            int ib, int jb, int cur, bool mirror, float* tile) {
+  const int lane = threadIdx.x & 63, h = lane >> 5, jl = lane & 31;
+  const int64_t xs = bt * 2 * M.mp * M.np, ss = bt * 2 * M.mp * M.mp;
+  float v[16];
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    f16x8 ph, pl;
+    if (EPI != NS_S) {
+      // the old S or X at [i][j]: R's fragment of row j (S is symmetric, R = Xt)
+      const _Float16* p = R + ns_blk(jb >> 5, (ib >> 4) + g, M.mp) + lane * 8;
+      ph = *(const f16x8*)p;
+      pl = *(const f16x8*)(p + 512);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float x = d[g * 8 + e] * o.up;
+      if (EPI != NS_S) x = fmaf(o.old, (float)ph[e] + (float)pl[e], x);
+      v[g * 8 + e] = x;
+    }
+  }
+  if (EPI == NS_LAST) {
+    const int64_t base = bt * M.rows * M.cols;
+    if (M.flip) {
+      // the caller's rows are j: through LDS, so that lanes run along i
+#pragma unroll
+      for (int e = 0; e < 16; ++e) tile[(8 * (e >> 2) + 4 * h + (e & 3)) * 33 + jl] = v[e];
+      ns_wave_sync();
+#pragma unroll
+      for (int e = 0; e < 16; ++e) v[e] = tile[jl * 33 + 2 * e + h];
+      ns_wave_sync();
+    }
+    // v[e] is the element (row, col) of the caller's matrix
+    const int col = (M.flip ? ib : jb) + jl;
+    if (col >= M.cols) return;
+    float w[16];
+    if (M.buf) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int row = M.flip ? jb + 2 * e + h : ib + 8 * (e >> 2) + 4 * h + (e & 3);
+        w[e] = row < M.rows ? ((const float*)M.out)[base + (int64_t)row * M.cols + col] : 0.f;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int row = M.flip ? jb + 2 * e + h : ib + 8 * (e >> 2) + 4 * h + (e & 3);
+      if (row >= M.rows) continue;
+      const int64_t at = base + (int64_t)row * M.cols + col;
+      const float x = o.down * v[e];
+      if (M.buf) ((float*)M.out)[at] = fmaf(sc.keep, w[e], x);
+      else if (M.dtype == SV2N_DT_F32) ((float*)M.out)[at] = x;
+      else if (M.dtype == SV2N_DT_BF16) ((__bf16*)M.out)[at] = (__bf16)x;
+      else ((_Float16*)M.out)[at] = (_Float16)x;
+    }
+    return;
+  }
+  // the transpose, rows j: straight from registers
+  _Float16* T = EPI == NS_S ? M.s + ss : EPI == NS_Q ? M.q + ss : M.xt[cur ^ 1] + xs;
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    f16x8 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      _Float16 a, b;
+      ns_split(v[g * 8 + e], a, b);
+      hi[e] = a;
+      lo[e] = b;
+    }
+    _Float16* p = T + ns_blk(jb >> 5, (ib >> 4) + g, M.mp) + lane * 8;
+    *(f16x8*)p = hi;
+    *(f16x8*)(p + 512) = lo;
+  }
+  if (!mirror) return;
+  // the tile itself, rows i
+#pragma unroll
+  for (int e = 0; e < 16; ++e) tile[(8 * (e >> 2) + 4 * h + (e & 3)) * 33 + jl] = v[e];
+  ns_wave_sync();
+  _Float16* D = EPI == NS_S ? M.s + ss : EPI == NS_Q ? M.q + ss : M.x + xs;
+  const int kd = EPI == NS_X ? M.np : M.mp;
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    f16x8 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      _Float16 a, b;
+      ns_split(tile[jl * 33 + 16 * g + ns_k(h, e)], a, b);
+      hi[e] = a;
+      lo[e] = b;
+    }
+    _Float16* p = D + ns_blk(ib >> 5, (jb >> 4) + g, kd) + lane * 8;
+    *(f16x8*)p = hi;
+    *(f16x8*)(p + 512) = lo;
+  }
+  ns_wave_sync();
+}
+
+// Blocks of a launch that share operand rows run on one XCD (its own L2): the
+// hardware deals blocks to the 8 XCDs in turn, so block b takes the (b / 8)-th tile of
+// the (b % 8)-th eighth.
+__device__ __forceinline__ int ns_xcd(int b, int n) {
+  const int x = b & 7, k = b >> 3, q = n >> 3, r = n & 7;
+  return x * q + min(x, r) + k;
+}
+
+struct NsTile {
+  const NsMat* M;
+  int bt, ti, tj;
+};
+// tile `b` (of TB x TB) of a launch
 template <int TB, int EPI>
-__global__ __launch_bounds__(256, 2) void k_ns_gemm(NsArgs A, NsScale sc, int cur) {
-  constexpr int WT = TB / 2, FT = WT / 32;
-  constexpr int OPB = TB * 128;              // bytes of an operand's stage
-  constexpr int LD = TB * 8 / 256;           // 16-B loads per thread and operand
-  __shared__ __attribute__((aligned(16))) char lds[2 * 2 * OPB];
-  const int mi = ns_find(A, blockIdx.x);
+__device__ __forceinline__ NsTile ns_tile_of(const NsArgs& A, int b) {
+  NsTile r;
+  const int mi = ns_find(A, b);
   const NsMat& M = A.mat[mi];
-  int local = blockIdx.x - A.first[mi];
+  int local = b - A.first[mi];
   const int tm = M.mp / TB, tn = M.np / TB;
-  int ti, tj;
-  int bt;
   if (EPI == NS_S || EPI == NS_Q) {
     const int per = tm * (tm + 1) / 2;
-    bt = local / per;
-    local -= bt * per;
-    ti = (int)((sqrtf(8.f * (float)local + 1.f) - 1.f) * 0.5f);
+    r.bt = local / per;
+    local -= r.bt * per;
+    int ti = (int)((sqrtf(8.f * (float)local + 1.f) - 1.f) * 0.5f);
     while (ti * (ti + 1) / 2 > local) --ti;
     while ((ti + 1) * (ti + 2) / 2 <= local) ++ti;
-    tj = local - ti * (ti + 1) / 2;
+    r.ti = ti;
+    r.tj = local - ti * (ti + 1) / 2;
   } else {
     const int per = tm * tn;
-    bt = local / per;
-    local -= bt * per;
-    ti = local % tm;
-    tj = local / tm;
+    r.bt = local / per;
+    local -= r.bt * per;
+    // strips of 8 rows of tiles, column by column
+    const int s0 = local / (8 * tn) * 8, sh = min(8, tm - s0);
+    local -= s0 * tn;
+    r.ti = s0 + local % sh;
+    r.tj = local / sh;
   }
-  const int i0 = ti * TB, j0 = tj * TB;
-  const int64_t xs = (int64_t)bt * 2 * M.mp * M.np, ss = (int64_t)bt * 2 * M.mp * M.mp;
-  const int kp = EPI == NS_S ? M.np : M.mp;
-  const _Float16* P = (EPI == NS_S ? M.x + xs : EPI == NS_Q ? M.s + ss : M.q + ss);
-  const _Float16* R = (EPI == NS_S ? M.x + xs : EPI == NS_Q ? M.s + ss : M.xt[cur] + xs);
+  r.M = &M;
+  return r;
+}
 
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const int wi = (wave >> 1) * WT, wj = (wave & 1) * WT;
-  const char* gp[LD];
-  const char* gr[LD];
-#pragma unroll
-  for (int l = 0; l < LD; ++l) {
-    const int q = l * 256 + t, row = q >> 3, g = (q & 7) ^ ((row >> 1) & 7);
-    gp[l] = (const char*)P + (int64_t)(i0 + row) * kp * 4 + g * 16;
-    gr[l] = (const char*)R + (int64_t)(j0 + row) * kp * 4 + g * 16;
+// The three (or, PR = 1, one) f16 products of a pair of fragments
+template <int PR>
+__device__ __forceinline__ f32x16 ns_mfma(const f16x8* a, const f16x8* b, f32x16 c) {
+  c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], b[0], c, 0, 0, 0);
+  if (PR == 3) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], b[1], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1], b[0], c, 0, 0, 0);
   }
-  u32x4 sp[LD], sr[LD];
+  return c;
+}
+
+// ---- 3a: a product over many tiles ----
+// 128 x 128 tiles, four waves of 64 x 64, two blocks a CU.  A stage is 16 KiB of an
+// operand (32 K values of both planes, 64 of the hi plane alone), staged through
+// registers into one of two LDS buffers: the next stage's loads are in flight while
+// this one is multiplied, one barrier a stage.
+template <int EPI, int PR>
+__global__ __launch_bounds__(256, 2) void k_ns_big(NsArgs A, NsScale sc, int cur) {
+  constexpr int OPH = 8192;                  // halves of an operand's stage
+  constexpr int KS = PR == 3 ? 2 : 4;        // 16-deep blocks of a stage
+  constexpr int PL = PR == 3 ? 2 : 1;        // planes read
+  __shared__ __attribute__((aligned(16))) _Float16 lds[4 * OPH];
+  const NsTile tl = ns_tile_of<128, EPI>(A, ns_xcd(blockIdx.x, gridDim.x));
+  const NsMat& M = *tl.M;
+  const int64_t xs = (int64_t)tl.bt * 2 * M.mp * M.np, ss = (int64_t)tl.bt * 2 * M.mp * M.mp;
+  const int kp = EPI == NS_S ? M.np : M.mp;
+  const _Float16* P = EPI == NS_S ? M.x + xs : EPI == NS_Q ? M.s + ss : M.q + ss;
+  const _Float16* R = EPI == NS_S ? M.x + xs : EPI == NS_Q ? M.s + ss : M.xt[cur] + xs;
+  const int t = threadIdx.x, lane = t & 63, wave = wave_id();
+  const int wi = wave >> 1, wj = wave & 1;
+  // thread t copies 16 B of each of the 4 row groups' 4 KiB
+  const int from = PR == 3 ? t * 8 : (t >> 6) * 1024 + lane * 8;
+  const _Float16* gp = P + ns_blk(tl.ti * 4, 0, kp) + from;
+  const _Float16* gr = R + ns_blk(tl.tj * 4, 0, kp) + from;
+  const int64_t rg = (int64_t)(kp >> 4) << 10;
+  u32x4 sp[4], sr[4];
   auto fetch = [&](int st) {
 #pragma unroll
-    for (int l = 0; l < LD; ++l) {
-      sp[l] = *(const u32x4*)(gp[l] + (int64_t)st * 128);
-      sr[l] = *(const u32x4*)(gr[l] + (int64_t)st * 128);
+    for (int l = 0; l < 4; ++l) {
+      sp[l] = *(const u32x4*)(gp + l * rg + (int64_t)st * (KS * 1024));
+      sr[l] = *(const u32x4*)(gr + l * rg + (int64_t)st * (KS * 1024));
     }
   };
   auto put = [&](int buf) {
 #pragma unroll
-    for (int l = 0; l < LD; ++l) {
-      *(u32x4*)(lds + buf * 2 * OPB + (l * 256 + t) * 16) = sp[l];
-      *(u32x4*)(lds + buf * 2 * OPB + OPB + (l * 256 + t) * 16) = sr[l];
+    for (int l = 0; l < 4; ++l) {
+      *(u32x4*)(lds + buf * 2 * OPH + l * 2048 + t * 8) = sp[l];
+      *(u32x4*)(lds + buf * 2 * OPH + OPH + l * 2048 + t * 8) = sr[l];
     }
   };
+  f32x16 acc[2][2];
+#pragma unroll
+  for (int x = 0; x < 2; ++x)
+#pragma unroll
+    for (int y = 0; y < 2; ++y)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[x][y][e] = 0.f;
+  const int nst = kp / (16 * KS);
+  fetch(0);
+  put(0);
+  __syncthreads();
+  for (int s = 0; s < nst; ++s) {
+    const bool more = s + 1 < nst;
+    if (more) fetch(s + 1);
+    const _Float16* bp = lds + (s & 1) * 2 * OPH + lane * 8;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      f16x8 a[2][2], b[2][2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int p = 0; p < PL; ++p) {
+          a[x][p] = *(const f16x8*)(bp + (wi * 2 + x) * 2048 + (k * PL + p) * 512);
+          b[x][p] = *(const f16x8*)(bp + OPH + (wj * 2 + x) * 2048 + (k * PL + p) * 512);
+        }
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) acc[x][y] = ns_mfma<PR>(a[x], b[y], acc[x][y]);
+    }
+    if (more) put((s & 1) ^ 1);
+    __syncthreads();
+  }
+  const NsOut o = ns_out<EPI>(sc, M);
+  float* tile = (float*)lds + wave * 32 * 33;
+#pragma unroll
+  for (int x = 0; x < 2; ++x)
+#pragma unroll
+    for (int y = 0; y < 2; ++y)
+      ns_epilogue<EPI>(acc[x][y], o, M, sc, R, tl.bt, tl.ti * 128 + wi * 64 + x * 32,
+                       tl.tj * 128 + wj * 64 + y * 32, cur, EPI == NS_X || tl.ti != tl.tj, tile);
+}
+
+// ---- 3b: a product over few tiles ----
+// Tiles of 32·FT a side; each of the block's W waves takes every W-th 16 K values of
+// the whole tile, fragments straight from memory into registers (DEPTH steps ahead),
+// no barrier until the W sums are added at the end in wave order.  big0 >= 0 (FT = 2):
+// the blocks are quarters of the 128 x 128 tiles from big0 on, what k_ns_big left.
+template <int EPI, int FT, int W, int PR>
+__global__ __launch_bounds__(64 * W, 2) void k_ns_small(NsArgs A, NsScale sc, int cur, int big0) {
+  constexpr int DEPTH = FT == 2 ? 3 : 5;
+  constexpr int PL = PR == 3 ? 2 : 1;
+  constexpr int TB = 32 * FT;
+  __shared__ float sum[FT * FT][W][16][64];  // [place][wave][element][lane]
+  const int bx = ns_xcd(blockIdx.x, gridDim.x);
+  NsTile tl;
+  if (FT == 2 && big0 >= 0) {
+    tl = ns_tile_of<128, EPI>(A, big0 + (bx >> 2));
+    const int si = (bx >> 1) & 1, sj = bx & 1;
+    // above the diagonal: its mirror's block writes it
+    if ((EPI == NS_S || EPI == NS_Q) && tl.ti == tl.tj && sj > si) return;
+    tl.ti = tl.ti * 2 + si;
+    tl.tj = tl.tj * 2 + sj;
+  } else {
+    tl = ns_tile_of<TB, EPI>(A, bx);
+  }
+  const NsMat& M = *tl.M;
+  const int64_t xs = (int64_t)tl.bt * 2 * M.mp * M.np, ss = (int64_t)tl.bt * 2 * M.mp * M.mp;
+  const int kp = EPI == NS_S ? M.np : M.mp;
+  const _Float16* P = EPI == NS_S ? M.x + xs : EPI == NS_Q ? M.s + ss : M.q + ss;
+  const _Float16* R = EPI == NS_S ? M.x + xs : EPI == NS_Q ? M.s + ss : M.xt[cur] + xs;
+  const int lane = threadIdx.x & 63, wave = wave_id();
+  const int64_t rg = (int64_t)(kp >> 4) << 10;
+  const _Float16* gp = P + ns_blk(tl.ti * FT, 0, kp) + lane * 8;
+  const _Float16* gr = R + ns_blk(tl.tj * FT, 0, kp) + lane * 8;
+  f16x8 a[DEPTH][FT][2], b[DEPTH][FT][2];
   f32x16 acc[FT][FT];
 #pragma unroll
   for (int x = 0; x < FT; ++x)
@@ -297,116 +542,97 @@ __global__ __launch_bounds__(256, 2) void k_ns_gemm(NsArgs A, NsScale sc, int cu
     for (int y = 0; y < FT; ++y)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[x][y][e] = 0.f;
-
-  auto frag = [&](int buf, int op, int row, int plane, int ks) {
-    const int slot = (plane * 4 + ks * 2 + (lane >> 5)) ^ ((row >> 1) & 7);
-    return *(const f16x8*)(lds + buf * 2 * OPB + op * OPB + row * 128 + slot * 16);
-  };
-  const int nst = kp / 32;
-  fetch(0);
-  put(0);
-  __syncthreads();
-  for (int st = 0; st < nst; ++st) {
-    const int buf = st & 1;
-    if (st + 1 < nst) fetch(st + 1);
+  const int nk = kp / 16;
+  auto fetch = [&](int d, int k) {
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      f16x8 ah[FT], al[FT], bh[FT], bl[FT];
+    for (int x = 0; x < FT; ++x)
 #pragma unroll
-      for (int x = 0; x < FT; ++x) {
-        const int ra = wi + x * 32 + (lane & 31), rb = wj + x * 32 + (lane & 31);
-        ah[x] = frag(buf, 0, ra, 0, ks);
-        bh[x] = frag(buf, 1, rb, 0, ks);
-        al[x] = frag(buf, 0, ra, 1, ks);
-        bl[x] = frag(buf, 1, rb, 1, ks);
+      for (int p = 0; p < PL; ++p) {
+        a[d][x][p] = *(const f16x8*)(gp + x * rg + (int64_t)k * 1024 + p * 512);
+        b[d][x][p] = *(const f16x8*)(gr + x * rg + (int64_t)k * 1024 + p * 512);
       }
+  };
+  auto mul = [&](int d) {
 #pragma unroll
-      for (int x = 0; x < FT; ++x)
+    for (int x = 0; x < FT; ++x)
 #pragma unroll
-        for (int y = 0; y < FT; ++y) {
-          acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[x], bh[y], acc[x][y], 0, 0, 0);
-          acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[x], bl[y], acc[x][y], 0, 0, 0);
-          acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[x], bh[y], acc[x][y], 0, 0, 0);
-        }
+      for (int y = 0; y < FT; ++y) acc[x][y] = ns_mfma<PR>(a[d][x], b[d][y], acc[x][y]);
+  };
+  // loads past the operand's end read its last block again (not used): without a
+  // branch the waits count the loads in flight
+#pragma unroll
+  for (int d = 0; d < DEPTH; ++d) fetch(d, min(wave + d * W, nk - 1));
+  int k = wave;
+  for (; k + (DEPTH - 1) * W < nk; k += DEPTH * W) {
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+      // (the scheduler would sink the loads to their use, and the distance with them)
+      __builtin_amdgcn_sched_barrier(0);
+      mul(d);
+      __builtin_amdgcn_sched_barrier(0);
+      fetch(d, min(k + (d + DEPTH) * W, nk - 1));
     }
-    if (st + 1 < nst) put(buf ^ 1);
-    __syncthreads();
   }
-
-  // epilogue: lane holds column j = lane & 31 and, in fours, rows i of each tile
-  float* tile = (float*)lds + wave * 32 * 33;
-  const float up_s = ldexpf(1.f, sc.ks - 2 * sc.kx);           // D of X Xt -> S's scale
-  const float up_q = sc.c * ldexpf(1.f, sc.kq - 2 * sc.ks);    // c·D of S S -> Q's scale
-  const float up_b = sc.b * ldexpf(1.f, sc.kq - sc.ks);
-  const float up_x = ldexpf(1.f, -sc.kq);                      // D of Q X -> X's scale
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int d = 0; d < DEPTH - 1; ++d)
+    if (k + d * W < nk) mul(d);
 #pragma unroll
   for (int x = 0; x < FT; ++x)
 #pragma unroll
-    for (int y = 0; y < FT; ++y) {
-      const int ib = i0 + wi + x * 32, jb = j0 + wj + y * 32;
-      const int il = 4 * (lane >> 5), jl = lane & 31;
+    for (int y = 0; y < FT; ++y)
 #pragma unroll
-      for (int r4 = 0; r4 < 4; ++r4) {
-        f16x4 ph, pl;
-        if (EPI != NS_S) {
-          // the old S or X at [i..i+3][j]: four values in a row of the (symmetric)
-          // S, or of Xt
-          const _Float16* o = R + ns_off(jb + jl, ib + 8 * r4 + il, kp);
-          ph = *(const f16x4*)o;
-          pl = *(const f16x4*)(o + 32);
-        }
+      for (int e = 0; e < 16; ++e) sum[x * FT + y][wave][e][lane] = acc[x][y][e];
+  __syncthreads();
+  f32x16 d;
+  float* tile;
+  int x = 0, y = 0;
+  if constexpr (FT == 2) {
+    // wave w finishes the tile at (w / 2, w % 2)
+    static_assert(W == 4, "one wave per place");
+    x = wave >> 1;
+    y = wave & 1;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float v = acc[x][y][r4 * 4 + e];
-          if (EPI == NS_S) {
-            v *= up_s;
-          } else {
-            const float old = (float)ph[e] + (float)pl[e];
-            if (EPI == NS_Q) v = fmaf(up_q, v, up_b * old);
-            else v = fmaf(up_x, v, sc.a * old);
-          }
-          tile[(8 * r4 + il + e) * 33 + jl] = v;
-        }
-      }
-      ns_wave_sync();  // the tile is the wave's own
-      if (EPI == NS_S || EPI == NS_Q) {
-        _Float16* D = (EPI == NS_S ? M.s : M.q) + ss;
-        ns_store<false>(tile, D, ib, jb, M.mp);
-        if (ti != tj) ns_store<true>(tile, D, jb, ib, M.mp);
-      } else if (EPI == NS_X) {
-        ns_store<false>(tile, M.x + xs, ib, jb, M.np);
-        ns_store<true>(tile, M.xt[cur ^ 1] + xs, jb, ib, M.mp);
-      } else {
-        const float down = ldexpf(1.f, -sc.kx);
-        const float f = M.buf ? -M.lr * down : down;
-        // along the caller's rows: 32 lanes a row, two rows at a time
-#pragma unroll 4
-        for (int p = 0; p < 16; ++p) {
-          const int u = 2 * p + (lane >> 5), v = lane & 31;
-          const int i = M.flip ? ib + v : ib + u, j = M.flip ? jb + u : jb + v;
-          if (i >= M.m || j >= M.n) continue;
-          const float val = f * (M.flip ? tile[v * 33 + u] : tile[u * 33 + v]);
-          const int64_t o = (int64_t)bt * M.rows * M.cols +
-                            (M.flip ? (int64_t)j * M.cols + i : (int64_t)i * M.cols + j);
-          if (M.buf) {
-            float* w = (float*)M.out + o;
-            *w = fmaf(sc.keep, *w, val);
-          } else if (M.dtype == SV2N_DT_F32) {
-            ((float*)M.out)[o] = val;
-          } else if (M.dtype == SV2N_DT_BF16) {
-            ((__bf16*)M.out)[o] = (__bf16)val;
-          } else {
-            ((_Float16*)M.out)[o] = (_Float16)val;
-          }
-        }
-      }
-      ns_wave_sync();
+    for (int e = 0; e < 16; ++e)
+      d[e] = (sum[wave][0][e][lane] + sum[wave][1][e][lane]) +
+             (sum[wave][2][e][lane] + sum[wave][3][e][lane]);
+    ns_wave_sync();
+    tile = &sum[wave][0][0][0];
+  } else {
+    // the waves add 16 / W elements each, the first one finishes the tile
+    constexpr int EW = 16 / W;
+    float part[EW];
+#pragma unroll
+    for (int q = 0; q < EW; ++q) {
+      part[q] = 0.f;
+#pragma unroll
+      for (int u = 0; u < W; ++u) part[q] += sum[0][u][wave * EW + q][lane];
     }
+    // slot 0 of an element is read by its own adder alone
+#pragma unroll
+    for (int q = 0; q < EW; ++q) sum[0][0][wave * EW + q][lane] = part[q];
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) d[e] = sum[0][0][e][lane];
+    ns_wave_sync();
+    tile = &sum[0][1][0][0];
+  }
+  const NsOut o = ns_out<EPI>(sc, M);
+  ns_epilogue<EPI>(d, o, M, sc, R, tl.bt, tl.ti * TB + x * 32, tl.tj * TB + y * 32, cur,
+                   EPI == NS_X || tl.ti != tl.tj, tile);
 }
 
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
+#ifndef SV2N_NS_BIG
+#define SV2N_NS_BIG 512
+#endif
+#ifndef SV2N_NS_TINY
+#define SV2N_NS_TINY 64
+#endif
+
 static inline int64_t ns_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 
 // Largest |f| of f(x) = x·p(x²) and of q(λ) = b λ + c λ² over [0, hi]: both are
@@ -457,28 +683,28 @@ static bool ns_scales(int steps, NsScale* sc) {
   return true;
 }
 
-// Tile of a group of matrices: 128 where that leaves at least 128 blocks for X's
-// product, else 64 (more blocks, each with half the K-loop's work per stage)
-static int ns_tile(const NsMat* mats, int count) {
-  int64_t blocks = 0;
-  for (int i = 0; i < count; ++i)
-    blocks += (int64_t)mats[i].batch * (ns_up(mats[i].m, 128) / 128) * (ns_up(mats[i].n, 128) / 128);
-  return blocks >= 128 ? 128 : 64;
-}
-
 static void ns_shape(NsMat* M) {
   M->flip = M->rows > M->cols;
   M->m = std::min(M->rows, M->cols);
   M->n = std::max(M->rows, M->cols);
-  int64_t pr = (NS_PART_ELEMS + M->cols - 1) / M->cols;
-  pr = std::max<int64_t>(pr, (M->rows + NS_PARTS - 1) / NS_PARTS);
-  M->part_rows = (int)std::min<int64_t>(pr, M->rows);
-  M->parts = (M->rows + M->part_rows - 1) / M->part_rows;
+  const int64_t total = (int64_t)M->rows * M->cols;
+  const int64_t each = std::max<int64_t>(NS_PART_ELEMS, (total + NS_PARTS - 1) / NS_PARTS);
+  M->part_elems = (int)ns_up(each, 8);
+  M->parts = (int)((total + M->part_elems - 1) / M->part_elems);
 }
 
-// pads the shapes for the group's tile and lays its workspace out from `ws`
+// What a group's matrices are padded to: 128 where some product fills the chip with
+// 128 x 128 tiles (X's, the largest), else 64
+static int ns_pad(const NsMat* mats, int count) {
+  int64_t tiles = 0;
+  for (int i = 0; i < count; ++i)
+    tiles += (int64_t)mats[i].batch * (ns_up(mats[i].m, 128) / 128) * (ns_up(mats[i].n, 128) / 128);
+  return tiles > SV2N_NS_BIG * 3 / 4 ? 128 : 64;
+}
+
+// pads the shapes and lays its workspace out from `ws`
 // (NULL: only counts); returns the bytes
-static int64_t ns_plan(NsMat* mats, int count, int tile, char* ws) {
+static int64_t ns_plan(NsMat* mats, int count, int pad, char* ws) {
   int64_t off = 0;
   auto take = [&](int64_t bytes) {
     char* p = ws ? ws + off : nullptr;
@@ -487,8 +713,8 @@ static int64_t ns_plan(NsMat* mats, int count, int tile, char* ws) {
   };
   for (int i = 0; i < count; ++i) {
     NsMat& M = mats[i];
-    M.mp = (int)ns_up(M.m, tile);
-    M.np = (int)ns_up(M.n, tile);
+    M.mp = (int)ns_up(M.m, pad);
+    M.np = (int)ns_up(M.n, pad);
     const int64_t xb = (int64_t)M.batch * M.mp * M.np * 4, sb = (int64_t)M.batch * M.mp * M.mp * 4;
     M.part = (double*)take((int64_t)M.batch * M.parts * 8);
     M.x = (_Float16*)take(xb);
@@ -511,33 +737,78 @@ static int64_t ns_blocks(NsArgs& A, F&& per) {
   return n;
 }
 
-template <int TB, int EPI>
-static void ns_gemm(NsArgs& A, const NsScale& sc, int cur, hipStream_t stream) {
-  const int64_t n = ns_blocks(A, [](const NsMat& M) -> int64_t {
-    const int64_t tm = M.mp / TB, tn = M.np / TB;
+template <int EPI>
+static int64_t ns_count(NsArgs& A, int tile) {
+  return ns_blocks(A, [&](const NsMat& M) -> int64_t {
+    const int64_t tm = M.mp / tile, tn = M.np / tile;
     return EPI == NS_S || EPI == NS_Q ? tm * (tm + 1) / 2 : tm * tn;
   });
-  hipLaunchKernelGGL((k_ns_gemm<TB, EPI>), dim3((unsigned)n), dim3(256), 0, stream, A, sc, cur);
 }
 
-template <int TB>
-static void ns_steps(NsArgs& A, const NsScale& sc, int steps, hipStream_t stream) {
-  for (int s = 0; s < steps; ++s) {
-    const int cur = s & 1;
-    ns_gemm<TB, NS_S>(A, sc, cur, stream);
-    ns_gemm<TB, NS_Q>(A, sc, cur, stream);
-    if (s + 1 < steps) ns_gemm<TB, NS_X>(A, sc, cur, stream);
-    else ns_gemm<TB, NS_LAST>(A, sc, cur, stream);
+template <int EPI, int PR>
+static void ns_product(NsArgs& A, const NsScale& sc, int cur, int pad, hipStream_t stream) {
+  if (pad == 128) {
+    // whole rounds of two blocks a CU; the rest on smaller tiles, or with them if the
+    // rest nearly fills a round
+    const int64_t n = ns_count<EPI>(A, 128);
+    int64_t big = n / SV2N_NS_BIG * SV2N_NS_BIG;
+    if (n - big > SV2N_NS_BIG * 3 / 4) big = n;
+    if (big > 0) {
+      hipLaunchKernelGGL((k_ns_big<EPI, PR>), dim3((unsigned)big), dim3(256), 0, stream, A, sc, cur);
+      if (n > big)
+        hipLaunchKernelGGL((k_ns_small<EPI, 2, 4, PR>), dim3((unsigned)(4 * (n - big))), dim3(256),
+                           0, stream, A, sc, cur, (int)big);
+      return;
+    }
+  }
+  const int64_t n = ns_count<EPI>(A, 64);
+  if (n >= SV2N_NS_TINY) {
+    hipLaunchKernelGGL((k_ns_small<EPI, 2, 4, PR>), dim3((unsigned)n), dim3(256), 0, stream, A, sc,
+                       cur, -1);
+  } else {
+    const int64_t n32 = ns_count<EPI>(A, 32);
+    hipLaunchKernelGGL((k_ns_small<EPI, 1, 8, PR>), dim3((unsigned)n32), dim3(512), 0, stream, A,
+                       sc, cur, -1);
   }
 }
 
-static int ns_run(NsArgs& A, const NsScale& sc, int steps, int tile, hipStream_t stream) {
+template <int PR>
+static void ns_one_step(NsArgs& A, const NsScale& sc, int s, bool last, int pad,
+                        hipStream_t stream) {
+  const int cur = s & 1;
+  ns_product<NS_S, PR>(A, sc, cur, pad, stream);
+  ns_product<NS_Q, PR>(A, sc, cur, pad, stream);
+  if (last) ns_product<NS_LAST, PR>(A, sc, cur, pad, stream);
+  else ns_product<NS_X, PR>(A, sc, cur, pad, stream);
+}
+
+// Steps at the start that may use the hi planes alone, where the result is bf16: with
+// |X|_F = 1 the singular values of an m-row matrix are about 1/sqrt(m), so S and Q are
+// a small correction to a X there (which keeps both planes) and their 2^-12 roundings
+// stay far below the result's 2^-9.  Measured against 64 bits (random, low-rank and
+// gradient-like matrices): the bf16 result's error grows by 0-1 % with 2 such steps
+// from m = 128 and by 0-5 % with 3 from m = 1,024; 16-row matrices would lose 27 %.
+static int ns_cheap(const NsMat& M, const NsScale& sc, int steps) {
+  if (M.dtype != SV2N_DT_BF16 || std::fabs(sc.a) > 4.f) return 0;
+  const int h = M.m >= 1024 ? 3 : M.m >= 128 ? 2 : 0;
+  return std::max(0, std::min(h, steps - 2));
+}
+
+static int ns_run(NsArgs& A, const NsScale& sc, int steps, int pad, hipStream_t stream) {
   int64_t n = ns_blocks(A, [](const NsMat& M) -> int64_t { return M.parts; });
-  hipLaunchKernelGGL(k_ns_norm, dim3((unsigned)n), dim3(256), 0, stream, A, sc);
+  const int dtype = A.mat[0].dtype;  // one for the whole group
+  auto* norm = dtype == SV2N_DT_F32 ? k_ns_norm<float>
+             : dtype == SV2N_DT_BF16 ? k_ns_norm<__bf16> : k_ns_norm<_Float16>;
+  auto* split = dtype == SV2N_DT_F32 ? k_ns_split<float>
+              : dtype == SV2N_DT_BF16 ? k_ns_split<__bf16> : k_ns_split<_Float16>;
+  hipLaunchKernelGGL(norm, dim3((unsigned)n), dim3(256), 0, stream, A, sc);
   n = ns_blocks(A, [](const NsMat& M) -> int64_t { return (int64_t)(M.mp / 64) * (M.np / 64); });
-  hipLaunchKernelGGL(k_ns_split, dim3((unsigned)n), dim3(256), 0, stream, A, sc);
-  if (tile == 128) ns_steps<128>(A, sc, steps, stream);
-  else ns_steps<64>(A, sc, steps, stream);
+  hipLaunchKernelGGL(split, dim3((unsigned)n), dim3(256), 0, stream, A, sc);
+  const int cheap = ns_cheap(A.mat[0], sc, steps);  // (16-bit types come one matrix a call)
+  for (int k = 0; k < steps; ++k) {
+    if (k < cheap) ns_one_step<1>(A, sc, k, false, pad, stream);
+    else ns_one_step<3>(A, sc, k, k + 1 == steps, pad, stream);
+  }
   return (int)hipGetLastError();
 }
 
@@ -561,7 +832,7 @@ extern "C" int64_t sv2n_orthogonalize_workspace(int64_t batch, int64_t rows, int
   M.cols = (int)cols;
   M.batch = (int)batch;
   ns_shape(&M);
-  return ns_plan(&M, 1, ns_tile(&M, 1), nullptr);
+  return ns_plan(&M, 1, ns_pad(&M, 1), nullptr);
 }
 
 extern "C" int sv2n_orthogonalize(const void* g, int64_t ld, int64_t batch_stride, int dtype,
@@ -582,11 +853,11 @@ extern "C" int sv2n_orthogonalize(const void* g, int64_t ld, int64_t batch_strid
   M.g = g; M.ld = ld; M.g_batch = batch_stride; M.out = out; M.dtype = dtype;
   M.rows = (int)rows; M.cols = (int)cols; M.batch = (int)batch;
   ns_shape(&M);
-  const int tile = ns_tile(&M, 1);
-  if (!workspace || workspace_bytes < ns_plan(&M, 1, tile, nullptr)) return SV2N_ERR_WORKSPACE;
+  const int pad = ns_pad(&M, 1);
+  if (!workspace || workspace_bytes < ns_plan(&M, 1, pad, nullptr)) return SV2N_ERR_WORKSPACE;
   if ((uintptr_t)workspace & 255) return SV2N_ERR_ALIGN;
-  ns_plan(&M, 1, tile, (char*)workspace);
-  return ns_run(A, sc, steps, tile, stream);
+  ns_plan(&M, 1, pad, (char*)workspace);
+  return ns_run(A, sc, steps, pad, stream);
 }
 
 // fills one group of at most NS_MAX matrices
@@ -617,7 +888,7 @@ extern "C" int64_t sv2n_muon_step_workspace(const sv2n_muon_matrix* mats, int co
       if (!ns_size_ok(1, mats[k + i].rows, mats[k + i].cols)) return 0;
     NsArgs A{};
     ns_group(mats + k, n, 0.0, &A);
-    most = std::max(most, ns_plan(A.mat, n, ns_tile(A.mat, n), nullptr));
+    most = std::max(most, ns_plan(A.mat, n, ns_pad(A.mat, n), nullptr));
   }
   return most;
 }
@@ -651,9 +922,9 @@ extern "C" int sv2n_muon_step(const sv2n_muon_matrix* mats, int count, double lr
     const int n = std::min(NS_MAX, count - k);
     NsArgs A{};
     ns_group(mats + k, n, lr, &A);
-    const int tile = ns_tile(A.mat, n);
-    ns_plan(A.mat, n, tile, (char*)workspace);
-    const int rc = ns_run(A, sc, steps, tile, stream);
+    const int pad = ns_pad(A.mat, n);
+    ns_plan(A.mat, n, pad, (char*)workspace);
+    const int rc = ns_run(A, sc, steps, pad, stream);
     if (rc) return rc;
   }
   return 0;

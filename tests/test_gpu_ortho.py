@@ -83,9 +83,37 @@ def test_flat_and_steep_spectra(dev):
     check((torch.mm(q1 * s, q2)).float())
 
 
-def test_large(dev):
-    check(gradient(dev, 2049, 1999))
-    check(gradient(dev, 16384, 96))
+@pytest.mark.parametrize("rows,cols,dtype", [
+    (2049, 1999, torch.float32), (16384, 96, torch.float32), (2600, 2570, torch.float32),
+    (3000, 3010, torch.float32), (4000, 4100, torch.float32), (4100, 4000, torch.bfloat16),
+    (2500, 3100, torch.bfloat16), (1100, 16000, torch.bfloat16)])
+def test_large(dev, rows, cols, dtype):
+    """Sizes past one round of 128 x 128 tiles, whole and with a remainder."""
+    check(gradient(dev, rows, cols, dtype))
+
+
+def test_large_stack(dev):
+    from spotv2net_amd import orthogonalize
+    g = torch.stack([gradient(dev, 1500, 1700, seed=k) for k in range(4)])
+    u = orthogonalize(g)
+    for k in range(4):
+        ref = definition(g[k])
+        assert rel(u[k], ref) <= allowed(g[k], ref), k
+
+
+def test_bf16_keeps_its_precision(dev):
+    """The bf16 path's cheaper first steps: the result is within 1.1 of what rounding
+    the exact one costs (2-norm), on flat, falling and nearly low-rank spectra."""
+    from spotv2net_amd import orthogonalize
+    gen = torch.Generator(device=dev).manual_seed(21)
+    for m, n in ((128, 300), (200, 3000), (512, 512), (1024, 1100), (1300, 5000)):
+        noise = torch.randn(m, n, device=dev, generator=gen)
+        low = torch.randn(m, 8, device=dev, generator=gen) @ \
+            torch.randn(8, n, device=dev, generator=gen)
+        for g in (noise, low + 0.05 * noise, gradient(dev, m, n)):
+            g = g.bfloat16()
+            ref = definition(g)
+            assert rel(orthogonalize(g), ref) <= 1.1 * rel(ref.bfloat16(), ref), (m, n)
 
 
 @pytest.mark.parametrize("co,steps", [((1.5, -0.5, 0.0), 20), ((15 / 8, -10 / 8, 3 / 8), 14)])
