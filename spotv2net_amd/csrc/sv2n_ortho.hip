@@ -42,6 +42,8 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 constexpr int NS_MAX = 16;      // matrices of one launch
 constexpr int NS_PARTS = 1024;  // most partial sums of squares of one matrix
 constexpr int NS_PART_ELEMS = 4096;
+constexpr int NS_HALF = 128;    // tiles of 128 that are worth a round of their own
+constexpr int NS_TINY = 72;     // tiles of 64 below which tiles of 32 are faster
 
 struct NsMat {
   const void* g;        // [batch][rows][ld] of dtype
@@ -420,99 +422,31 @@ __device__ __forceinline__ f32x16 ns_mfma(const f16x8* a, const f16x8* b, f32x16
   return c;
 }
 
-// ---- 3a: a product over many tiles ----
-// 128 x 128 tiles, four waves of 64 x 64, two blocks a CU.  A stage is 16 KiB of an
-// operand (32 K values of both planes, 64 of the hi plane alone), staged through
-// registers into one of two LDS buffers: the next stage's loads are in flight while
-// this one is multiplied, one barrier a stage.
-template <int EPI, int PR>
-__global__ __launch_bounds__(256, 2) void k_ns_big(NsArgs A, NsScale sc, int cur) {
-  constexpr int OPH = 8192;                  // halves of an operand's stage
-  constexpr int KS = PR == 3 ? 2 : 4;        // 16-deep blocks of a stage
-  constexpr int PL = PR == 3 ? 2 : 1;        // planes read
-  __shared__ __attribute__((aligned(16))) _Float16 lds[4 * OPH];
-  const NsTile tl = ns_tile_of<128, EPI>(A, ns_xcd(blockIdx.x, gridDim.x));
-  const NsMat& M = *tl.M;
-  const int64_t xs = (int64_t)tl.bt * 2 * M.mp * M.np, ss = (int64_t)tl.bt * 2 * M.mp * M.mp;
-  const int kp = EPI == NS_S ? M.np : M.mp;
-  const _Float16* P = EPI == NS_S ? M.x + xs : EPI == NS_Q ? M.s + ss : M.q + ss;
-  const _Float16* R = EPI == NS_S ? M.x + xs : EPI == NS_Q ? M.s + ss : M.xt[cur] + xs;
-  const int t = threadIdx.x, lane = t & 63, wave = wave_id();
-  const int wi = wave >> 1, wj = wave & 1;
-  // thread t copies 16 B of each of the 4 row groups' 4 KiB
-  const int from = PR == 3 ? t * 8 : (t >> 6) * 1024 + lane * 8;
-  const _Float16* gp = P + ns_blk(tl.ti * 4, 0, kp) + from;
-  const _Float16* gr = R + ns_blk(tl.tj * 4, 0, kp) + from;
-  const int64_t rg = (int64_t)(kp >> 4) << 10;
-  u32x4 sp[4], sr[4];
-  auto fetch = [&](int st) {
-#pragma unroll
-    for (int l = 0; l < 4; ++l) {
-      sp[l] = *(const u32x4*)(gp + l * rg + (int64_t)st * (KS * 1024));
-      sr[l] = *(const u32x4*)(gr + l * rg + (int64_t)st * (KS * 1024));
-    }
-  };
-  auto put = [&](int buf) {
-#pragma unroll
-    for (int l = 0; l < 4; ++l) {
-      *(u32x4*)(lds + buf * 2 * OPH + l * 2048 + t * 8) = sp[l];
-      *(u32x4*)(lds + buf * 2 * OPH + OPH + l * 2048 + t * 8) = sr[l];
-    }
-  };
-  f32x16 acc[2][2];
-#pragma unroll
-  for (int x = 0; x < 2; ++x)
-#pragma unroll
-    for (int y = 0; y < 2; ++y)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[x][y][e] = 0.f;
-  const int nst = kp / (16 * KS);
-  fetch(0);
-  put(0);
-  __syncthreads();
-  for (int s = 0; s < nst; ++s) {
-    const bool more = s + 1 < nst;
-    if (more) fetch(s + 1);
-    const _Float16* bp = lds + (s & 1) * 2 * OPH + lane * 8;
-#pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      f16x8 a[2][2], b[2][2];
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int p = 0; p < PL; ++p) {
-          a[x][p] = *(const f16x8*)(bp + (wi * 2 + x) * 2048 + (k * PL + p) * 512);
-          b[x][p] = *(const f16x8*)(bp + OPH + (wj * 2 + x) * 2048 + (k * PL + p) * 512);
-        }
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int y = 0; y < 2; ++y) acc[x][y] = ns_mfma<PR>(a[x], b[y], acc[x][y]);
-    }
-    if (more) put((s & 1) ^ 1);
-    __syncthreads();
-  }
-  const NsOut o = ns_out<EPI>(sc, M);
-  float* tile = (float*)lds + wave * 32 * 33;
-#pragma unroll
-  for (int x = 0; x < 2; ++x)
-#pragma unroll
-    for (int y = 0; y < 2; ++y)
-      ns_epilogue<EPI>(acc[x][y], o, M, sc, R, tl.bt, tl.ti * 128 + wi * 64 + x * 32,
-                       tl.tj * 128 + wj * 64 + y * 32, cur, EPI == NS_X || tl.ti != tl.tj, tile);
-}
-
-// ---- 3b: a product over few tiles ----
-// Tiles of 32·FT a side; each of the block's W waves takes every W-th 16 K values of
-// the whole tile, fragments straight from memory into registers (DEPTH steps ahead),
-// no barrier until the W sums are added at the end in wave order.  big0 >= 0 (FT = 2):
-// the blocks are quarters of the 128 x 128 tiles from big0 on, what k_ns_big left.
+// ---- 3: one product ----
+// Tiles of 32·FT a side.  Each of the block's W waves takes every W-th 16 K values of
+// the whole tile: fragments go straight from memory into registers, DEPTH steps
+// ahead, and nothing waits for another wave until the W sums are added at the end in
+// wave order.  The wider the wave's tile, the fewer bytes a product needs (FT = 1, 2,
+// 4: 4, 8, 16 KiB for 3, 12, 48 matrix instructions), so what bounds it goes from the
+// caches to the matrix cores, but the fewer blocks there are and the more the sums at
+// the end cost.  MI355X, one product of an f32 orthogonalisation, us:
+//                                        FT = 1    FT = 2    FT = 4
+//   X' of 512 x 512     (K 512)             6.1       7.5      17.9
+//   S of 1,024 x 4,096  (K 4,096)          44.2      27.7      61.9
+//   X' of 1,024 x 4,096 (K 1,024)          54.9      38.1      34.9
+//   X' of 2,048 x 2,048                       -      70.7      55.8
+//   X' of 4,096 x 4,096                       -       511       365   (1.13 Pflop/s of f16)
+// FT = 4 keeps 256 accumulators and two steps of fragments in the 512 registers of the
+// one wave per SIMD.  big0 >= 0 (FT = 2): the blocks are quarters of the 128 x 128 tiles
+// from big0 on, what whole rounds of FT = 4 left.
 template <int EPI, int FT, int W, int PR>
-__global__ __launch_bounds__(64 * W, 2) void k_ns_small(NsArgs A, NsScale sc, int cur, int big0) {
-  constexpr int DEPTH = FT == 2 ? 3 : 5;
+__global__ __launch_bounds__(64 * W, FT == 4 ? 1 : 2) void k_ns_mm(NsArgs A, NsScale sc, int cur, int big0) {
+  constexpr int DEPTH = FT == 4 ? (PR == 3 ? 2 : 4) : FT == 2 ? 3 : 5;
   constexpr int PL = PR == 3 ? 2 : 1;
   constexpr int TB = 32 * FT;
-  __shared__ float sum[FT * FT][W][16][64];  // [place][wave][element][lane]
+  // [place][wave][element][lane]; FT = 4: [owner of 2][wave][tile of 4][element][lane]
+  extern __shared__ float s_sum[];
+  auto sum = (float (*)[W][16][64])s_sum;
   const int bx = ns_xcd(blockIdx.x, gridDim.x);
   NsTile tl;
   if (FT == 2 && big0 >= 0) {
@@ -577,6 +511,43 @@ __global__ __launch_bounds__(64 * W, 2) void k_ns_small(NsArgs A, NsScale sc, in
 #pragma unroll
   for (int d = 0; d < DEPTH - 1; ++d)
     if (k + d * W < nk) mul(d);
+  if constexpr (FT == 4) {
+    // wave w finishes the 64 x 64 quadrant (w / 2, w % 2); two quadrants' sums at a
+    // time fit the LDS
+    const NsOut o = ns_out<EPI>(sc, M);
+    f32x16 own[2][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            s_sum[(((q * 4 + wave) * 4 + v) * 16 + e) * 64 + lane] =
+                acc[h * 2 + (v >> 1)][q * 2 + (v & 1)][e];
+      __syncthreads();
+      if ((wave >> 1) == h) {
+        const int q = wave & 1;
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float* c = s_sum + (((q * 4) * 4 + v) * 16 + e) * 64 + lane;
+            own[v >> 1][v & 1][e] = (c[0] + c[4096]) + (c[2 * 4096] + c[3 * 4096]);
+          }
+      }
+      __syncthreads();
+    }
+    float* tile = s_sum + wave * 32 * 33;
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+      ns_epilogue<EPI>(own[v >> 1][v & 1], o, M, sc, R, tl.bt,
+                       tl.ti * TB + (wave >> 1) * 64 + (v >> 1) * 32,
+                       tl.tj * TB + (wave & 1) * 64 + (v & 1) * 32, cur,
+                       EPI == NS_X || tl.ti != tl.tj, tile);
+    return;
+  } else {
 #pragma unroll
   for (int x = 0; x < FT; ++x)
 #pragma unroll
@@ -621,18 +592,12 @@ __global__ __launch_bounds__(64 * W, 2) void k_ns_small(NsArgs A, NsScale sc, in
   const NsOut o = ns_out<EPI>(sc, M);
   ns_epilogue<EPI>(d, o, M, sc, R, tl.bt, tl.ti * TB + x * 32, tl.tj * TB + y * 32, cur,
                    EPI == NS_X || tl.ti != tl.tj, tile);
+  }
 }
 
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
-#ifndef SV2N_NS_BIG
-#define SV2N_NS_BIG 512
-#endif
-#ifndef SV2N_NS_TINY
-#define SV2N_NS_TINY 64
-#endif
-
 static inline int64_t ns_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 
 // Largest |f| of f(x) = x·p(x²) and of q(λ) = b λ + c λ² over [0, hi]: both are
@@ -693,13 +658,16 @@ static void ns_shape(NsMat* M) {
   M->parts = (int)((total + M->part_elems - 1) / M->part_elems);
 }
 
-// What a group's matrices are padded to: 128 where some product fills the chip with
-// 128 x 128 tiles (X's, the largest), else 64
+// What a group's matrices are padded to: 128 where X's product (the largest) is worth
+// tiles of 128: enough of them, and at least 1,024 deep (K 777, 273 tiles: 47.4 us
+// against 31.8 on tiles of 64), else 64
 static int ns_pad(const NsMat* mats, int count) {
   int64_t tiles = 0;
   for (int i = 0; i < count; ++i)
-    tiles += (int64_t)mats[i].batch * (ns_up(mats[i].m, 128) / 128) * (ns_up(mats[i].n, 128) / 128);
-  return tiles > SV2N_NS_BIG * 3 / 4 ? 128 : 64;
+    if (mats[i].m >= 1024)
+      tiles += (int64_t)mats[i].batch * (ns_up(mats[i].m, 128) / 128) *
+               (ns_up(mats[i].n, 128) / 128);
+  return tiles >= NS_HALF ? 128 : 64;
 }
 
 // pads the shapes and lays its workspace out from `ws`
@@ -745,31 +713,35 @@ static int64_t ns_count(NsArgs& A, int tile) {
   });
 }
 
+template <int EPI, int FT, int W, int PR>
+static void ns_launch(NsArgs& A, const NsScale& sc, int cur, int64_t blocks, int big0,
+                      hipStream_t stream) {
+  constexpr int lds = FT == 4 ? 131072 : FT * FT * W * 4096;
+  auto* k = k_ns_mm<EPI, FT, W, PR>;
+  if (lds > 65536)
+    (void)hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(64 * W), lds, stream, A, sc, cur, big0);
+}
+
+// A product over the group's tiles.  Tiles of 128 where they fill at least half of the
+// chip's 256 CUs (one block each) in every round; fewer than that left over go on
+// tiles of 64, as do products that never have so many; tiles of 32 where even those
+// are under NS_TINY (the measured sides: k_ns_mm).
 template <int EPI, int PR>
 static void ns_product(NsArgs& A, const NsScale& sc, int cur, int pad, hipStream_t stream) {
   if (pad == 128) {
-    // whole rounds of two blocks a CU; the rest on smaller tiles, or with them if the
-    // rest nearly fills a round
     const int64_t n = ns_count<EPI>(A, 128);
-    int64_t big = n / SV2N_NS_BIG * SV2N_NS_BIG;
-    if (n - big > SV2N_NS_BIG * 3 / 4) big = n;
+    int64_t big = n / 256 * 256;
+    if (n - big >= NS_HALF) big = n;
     if (big > 0) {
-      hipLaunchKernelGGL((k_ns_big<EPI, PR>), dim3((unsigned)big), dim3(256), 0, stream, A, sc, cur);
-      if (n > big)
-        hipLaunchKernelGGL((k_ns_small<EPI, 2, 4, PR>), dim3((unsigned)(4 * (n - big))), dim3(256),
-                           0, stream, A, sc, cur, (int)big);
+      ns_launch<EPI, 4, 4, PR>(A, sc, cur, big, -1, stream);
+      if (n > big) ns_launch<EPI, 2, 4, PR>(A, sc, cur, 4 * (n - big), (int)big, stream);
       return;
     }
   }
   const int64_t n = ns_count<EPI>(A, 64);
-  if (n >= SV2N_NS_TINY) {
-    hipLaunchKernelGGL((k_ns_small<EPI, 2, 4, PR>), dim3((unsigned)n), dim3(256), 0, stream, A, sc,
-                       cur, -1);
-  } else {
-    const int64_t n32 = ns_count<EPI>(A, 32);
-    hipLaunchKernelGGL((k_ns_small<EPI, 1, 8, PR>), dim3((unsigned)n32), dim3(512), 0, stream, A,
-                       sc, cur, -1);
-  }
+  if (n >= NS_TINY) ns_launch<EPI, 2, 4, PR>(A, sc, cur, n, -1, stream);
+  else ns_launch<EPI, 1, 8, PR>(A, sc, cur, ns_count<EPI>(A, 32), -1, stream);
 }
 
 template <int PR>
