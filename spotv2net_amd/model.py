@@ -15,6 +15,8 @@ The GAT layers run as ONE fused autograd node (``stack.gat_stack``):
   model's activation and the inter-layer dropout (utils/models.py:147-148) in
   its epilogue; the final ``nn.Linear`` (:150) keeps its module and
   parameters but runs on the sv2n head kernels.
+``layer_norm=True`` (not in the reference) normalises every GAT layer's output
+with ``norm.LayerNorm`` inside the same node.
 Documented deviation: an unknown activation raises ValueError instead of
 printing and calling ``sys.exit()`` (utils/models.py:131-133).
 """
@@ -30,6 +32,7 @@ from . import graphed, ops
 from .conv import GATConv
 from .data import bf16_twin, twin_only_x
 from .layout import GraphLayout, analyze_edge_index, check_full_edge_attr, declare_canonical
+from .norm import LayerNorm
 from .stack import gat_stack, gat_train_head_mse, head_mse_loss, linear_head
 
 
@@ -83,7 +86,7 @@ def _layout_of(data, x: torch.Tensor, edge_index: torch.Tensor) -> GraphLayout:
 class GATModel(nn.Module):
     def __init__(self, num_node_features, num_edge_features, num_heads, output_node_channels,
                  dim_hidden_layers=[100], dropout_att=0.0, dropout=0.0, activation="relu",
-                 concat_heads=False, negative_slope=0.2, standardize=False):
+                 concat_heads=False, negative_slope=0.2, standardize=False, layer_norm=False):
         super().__init__()
         self.dropout = dropout
         self.activation = activation
@@ -107,6 +110,11 @@ class GATModel(nn.Module):
             stacked.append(GATConv(in_ch, dim_hidden_layers[i + 1],
                                    concat=(False if last else concat_heads), **kw))
         self.gat_layers = nn.ModuleList(first + stacked)
+        # layer_norm: every layer's output (after activation and dropout) is
+        # layer-normalised over its features, with a weight and bias of its own
+        self.norms = nn.ModuleList([
+            LayerNorm(c.heads * c.out_channels if c.concat else c.out_channels)
+            for c in self.gat_layers]) if layer_norm else None
         self.linear = nn.Linear(dim_hidden_layers[-1], output_node_channels)
 
         # execution mode of the GAT stack: None = fp32 unless inside
@@ -137,7 +145,7 @@ class GATModel(nn.Module):
             layout = _layout_of(data, x, edge_index)
         return gat_stack(x, edge_attr, tuple(self.gat_layers), layout, self._act_code,
                          float(self.dropout or 0.0), self.training, self.precision,
-                         None if self.standardize else bf16_twin(data))
+                         None if self.standardize else bf16_twin(data), self.norms)
 
     def _train_head_mse(self, data, target: torch.Tensor,
                         loss_sum: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
@@ -145,7 +153,7 @@ class GATModel(nn.Module):
         the MSE loss fused into the last GAT layer (stack.gat_train_head_mse):
         the loss, with every gradient accumulated into ``p.grad``; None when
         the model / batch does not take that path."""
-        if self.standardize or not self.training:
+        if self.standardize or self.norms is not None or not self.training:
             return None
         layout = _layout_of(data, data.x, data.edge_index)
         return gat_train_head_mse(data.x, data.edge_attr, tuple(self.gat_layers), layout,
@@ -162,7 +170,7 @@ class GATModel(nn.Module):
 
     def forward(self, data):
         layout = None
-        if self.graph_replay and not self.standardize:
+        if self.graph_replay and not self.standardize and self.norms is None:
             x, edge_index, edge_attr = data.x, data.edge_index, data.edge_attr
             layout = _layout_of(data, x, edge_index)
             out = graphed.forward(self, data, x, edge_index, edge_attr, layout)

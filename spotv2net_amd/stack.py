@@ -179,6 +179,11 @@ def layer_params(conv) -> list:
     return ps
 
 
+def norm_params(norms) -> list:
+    """The parameters of a stack's layer norms (none without norms)."""
+    return [p for m in norms or () for p in (m.weight, m.bias) if p is not None]
+
+
 def _ldx(conv) -> int:
     return (conv.heads * conv.out_channels + 2 * conv.heads + 3) // 4 * 4
 
@@ -343,7 +348,8 @@ HEAD_FUSE = os.environ.get("SV2N_HEAD_FUSE", "on")
 
 
 def stack_forward(x, edge_attr, convs, layout: GraphLayout, act: int, post_dropout: float,
-                  training: bool, precision: str, need_saved: bool, head=None, x_bf16=None):
+                  training: bool, precision: str, need_saved: bool, head=None, x_bf16=None,
+                  norms=None):
     """The fused stack's forward launches (module docstring); returns the
     output, the tensors the backward reads and a ``_StackMeta``.  Capturable:
     no host synchronisation, every buffer from the caching allocator.
@@ -352,7 +358,8 @@ def stack_forward(x, edge_attr, convs, layout: GraphLayout, act: int, post_dropo
     checked ``head_mse_fusable``); the output is then the loss and
     ``meta.head_dz`` the last layer's incoming gradient.  ``x_bf16``: bf16(x)
     from the data builder (data.bf16_twin), read by the bf16 mode's layer-0
-    GEMMs instead of rounding x."""
+    GEMMs instead of rounding x.  ``norms``: one LayerNorm module per layer,
+    applied to the layer's output (after its activation and dropout), or None."""
     ops = torch.ops.sv2n
     dev = x.device
     L = len(convs)
@@ -440,6 +447,7 @@ def stack_forward(x, edge_attr, convs, layout: GraphLayout, act: int, post_dropo
     xb0 = None  # bf16(x) of layer 0 (bf16 mode, x without grad)
     saved_x, saved_xs, saved_y, saved_p, saved_keep, saved_drop = [], [], [], [], [], []
     saved_st = []
+    saved_norm = []
     post_p = []
     for l, c in enumerate(convs):
         Hc, C = c.heads, c.out_channels
@@ -530,20 +538,24 @@ def stack_forward(x, edge_attr, convs, layout: GraphLayout, act: int, post_dropo
         saved_keep.append(keep)
         saved_drop.append(dmask)
         xin = out
+        if norms is not None:
+            xin, mean, rstd = ops.layer_norm(out, norms[l].weight, norms[l].bias, norms[l].eps)
+            saved_norm += [out, mean, rstd]
 
     meta = _StackMeta((L, act, use_edge, hp, H, eo, fused), bf16, feid,
                       [(1.0 / (1.0 - c.dropout)) if (training and 0.0 < c.dropout < 1.0) else
                        (0.0 if training and c.dropout >= 1.0 else 1.0) for c in convs], post_p,
                       saved_y[-1] if head is not None else None, cv)
     saved = [ea, wf if fused else None, *saved_x, *saved_xs, *saved_y, *saved_p, *saved_st,
-             *saved_keep, *saved_drop, *waugs, *planes_t, xb0]
+             *saved_keep, *saved_drop, *waugs, *planes_t, xb0, *saved_norm]
     return xin, saved, meta
 
 
 def stack_backward(saved, meta: _StackMeta, convs, layout: GraphLayout, dout, need_x0: bool,
-                   grad_of: "_GradTargets"):
+                   grad_of: "_GradTargets", norms=None):
     """The fused stack's backward launches, layers in reverse (module
-    docstring); parameter gradients go where ``grad_of`` says; returns dx."""
+    docstring); parameter gradients go where ``grad_of`` says; returns dx.
+    ``norms``: as in the forward."""
     ops = torch.ops.sv2n
     L, act, use_edge, hp, H, eo, fused = meta.dims
     sv = saved
@@ -559,6 +571,7 @@ def stack_backward(saved, meta: _StackMeta, convs, layout: GraphLayout, dout, ne
     waugs = sv[k:k + L]; k += L
     planes_t = sv[k:k + L]; k += L
     xb0 = sv[k]  # bf16(x) of layer 0, or None
+    normed = sv[k + 1:]  # per layer: the output before its norm, mean, rstd
     dev = dout.device
     B, n, N = layout.num_graphs, layout.n, layout.num_nodes
 
@@ -631,6 +644,10 @@ def stack_backward(saved, meta: _StackMeta, convs, layout: GraphLayout, dout, ne
     for l in range(L - 1, -1, -1):
         c = convs[l]
         Hc, C = c.heads, c.out_channels
+        if norms is not None:
+            dy = ops.layer_norm_bwd_acc(dy, normed[3 * l], norms[l].weight, normed[3 * l + 1],
+                                        normed[3 * l + 2], grad_of(norms[l].weight),
+                                        grad_of(norms[l].bias))
         post_u = drops[l] if meta.post_p[l] is not None else None
         if drops[l] is not None and post_u is None:
             dy = dy * drops[l]
@@ -698,8 +715,8 @@ def stack_backward(saved, meta: _StackMeta, convs, layout: GraphLayout, dout, ne
             # stores dZ = relu'(y)·dy itself (sv2n_gemm_f32x3_relu) and that
             # layer's attention backward runs with the identity (reads no y)
             relu_y = None
-            if l > 0 and act == ACT_RELU and not fused and not layout.tiled and \
-                    relu_mask_fusable(dxs, _opt(planes_t[l]), meta.bf16):
+            if l > 0 and act == ACT_RELU and norms is None and not fused and \
+                    not layout.tiled and relu_mask_fusable(dxs, _opt(planes_t[l]), meta.bf16):
                 relu_y, act_l = ys[l - 1], 0
             dy = ops.project(dxs, _opt(planes_t[l]), waugs[l], True, meta.bf16, relu_y)
 
@@ -714,11 +731,12 @@ def stack_backward(saved, meta: _StackMeta, convs, layout: GraphLayout, dout, ne
 class _GATStack(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, edge_attr, convs, layout: GraphLayout, act: int, post_dropout: float,
-                training: bool, precision: str, x_bf16, *params):
+                training: bool, precision: str, x_bf16, norms, *params):
         out, saved, meta = stack_forward(x, edge_attr, convs, layout, act, post_dropout, training,
                                          precision, training or any(ctx.needs_input_grad),
-                                         x_bf16=x_bf16)
+                                         x_bf16=x_bf16, norms=norms)
         ctx.convs = convs
+        ctx.norms = norms
         ctx.layout = layout
         ctx.direct = _direct_mode()
         ctx.meta = meta
@@ -727,11 +745,13 @@ class _GATStack(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dout):
-        params = [p for c in ctx.convs for p in layer_params(c)]
-        grad_of = _GradTargets(params, ctx.needs_input_grad[9:], ctx.direct, dout.device)
+        params = [p for c in ctx.convs for p in layer_params(c)] + norm_params(ctx.norms)
+        needs = [p.requires_grad for p in params] if ctx.direct else ctx.needs_input_grad[10:]
+        grad_of = _GradTargets(params, needs, ctx.direct, dout.device)
         dx0 = stack_backward(ctx.saved_tensors, ctx.meta, ctx.convs, ctx.layout, dout,
-                             ctx.needs_input_grad[0], grad_of)
-        return (dx0, None, None, None, None, None, None, None, None) + grad_of.returned()
+                             ctx.needs_input_grad[0], grad_of, ctx.norms)
+        return (dx0, None, None, None, None, None, None, None, None, None) + \
+            ((None,) if ctx.direct else grad_of.returned())
 
 
 def _a16_ok(x_bf16: torch.Tensor, xin: torch.Tensor, planes) -> bool:
@@ -844,9 +864,11 @@ def _require_params(params) -> None:
 
 def gat_stack(x: torch.Tensor, edge_attr: Optional[torch.Tensor], convs: Sequence,
               layout: GraphLayout, act: int, post_dropout: float, training: bool,
-              precision: Optional[str] = None,
-              x_bf16: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """Run ``convs`` (GATConv modules) as one fused autograd node.
+              precision: Optional[str] = None, x_bf16: Optional[torch.Tensor] = None,
+              norms: Optional[Sequence] = None) -> torch.Tensor:
+    """Run ``convs`` (GATConv modules) as one fused autograd node; with ``norms``
+    (a LayerNorm module per layer) each layer's output, after its activation and
+    dropout, is layer-normalised inside it.
 
     ``precision``: "f32" (f32-accurate GEMMs, 1e-5 parity with PyG fp32) or
     "bf16" (projection and weight-gradient GEMMs on bf16 operands with fp32
@@ -856,6 +878,7 @@ def gat_stack(x: torch.Tensor, edge_attr: Optional[torch.Tensor], convs: Sequenc
     params = []
     for c in convs:
         params += layer_params(c)
+    params += norm_params(norms)
     _require_params(params)
     _require_device(x, edge_attr)
     if edge_attr is not None and edge_attr.requires_grad:
@@ -864,8 +887,15 @@ def gat_stack(x: torch.Tensor, edge_attr: Optional[torch.Tensor], convs: Sequenc
     for p in params:
         if p.device != x.device:
             raise RuntimeError("parameters and data must be on the same device")
+    if _direct_mode():
+        # the gradients go straight to p.grad: an empty leaf stands for the parameters,
+        # so that the node has no edge to their accumulation nodes (an eager graph that
+        # is alive keeps those on its own stream, and a captured backward would wait for
+        # that stream)
+        params = [torch.empty(0, device=x.device, requires_grad=True)]
     out = _GATStack.apply(x, edge_attr, tuple(convs), layout, int(act), float(post_dropout),
-                          bool(training), precision, x_bf16, *params)
+                          bool(training), precision, x_bf16,
+                          None if norms is None else tuple(norms), *params)
     return layout.poison(out)  # NaN if a deferred layout check failed (layout.py)
 
 

@@ -29,29 +29,39 @@ import torch
 import torch.distributed as dist
 
 
-def flatten_params(params) -> torch.Tensor:
-    """Re-home every parameter as a view of ONE flat fp32 buffer (values kept)."""
-    params = [p for p in params if p.requires_grad]
-    flat = torch.cat([p.detach().reshape(-1) for p in params]).contiguous()
-    off = 0
+def _offsets(params, align: int):
+    """Where each parameter starts in a flat buffer (a multiple of ``align``
+    elements), and the buffer's length."""
+    offs, off = [], 0
     for p in params:
+        off = -(-off // align) * align
+        offs.append(off)
+        off += p.numel()
+    return offs, -(-off // align) * align
+
+
+def flatten_params(params, align: int = 1) -> torch.Tensor:
+    """Re-home every parameter as a view of ONE flat fp32 buffer (values kept),
+    each starting at a multiple of ``align`` elements (gaps are zero)."""
+    params = [p for p in params if p.requires_grad]
+    offs, total = _offsets(params, align)
+    flat = torch.zeros(total, device=params[0].device, dtype=params[0].dtype)
+    for p, off in zip(params, offs):
         k = p.numel()
+        flat[off:off + k].copy_(p.detach().reshape(-1))
         p.data = flat[off:off + k].view_as(p)
-        off += k
     return flat
 
 
-def flatten_grads(params) -> torch.Tensor:
-    """Allocate one flat buffer and make every ``p.grad`` a view into it."""
+def flatten_grads(params, align: int = 1) -> torch.Tensor:
+    """Allocate one flat buffer and make every ``p.grad`` a view into it (laid out
+    as ``flatten_params``)."""
     params = [p for p in params if p.requires_grad]
-    total = sum(p.numel() for p in params)
-    dev = params[0].device
-    flat = torch.zeros(total, device=dev, dtype=torch.float32)
-    off = 0
-    for p in params:
+    offs, total = _offsets(params, align)
+    flat = torch.zeros(total, device=params[0].device, dtype=torch.float32)
+    for p, off in zip(params, offs):
         k = p.numel()
         p.grad = flat[off:off + k].view_as(p)
-        off += k
     return flat
 
 
@@ -72,10 +82,71 @@ class FlatAdam:
     # the kernel advances step_t itself and zeroes the consumed gradient
     zeroes_grads = True
 
+    def state(self) -> list:
+        """Every tensor a step advances besides the parameters."""
+        return [self.m, self.v, self.step_t]
+
     def step(self) -> None:
         torch.ops.sv2n.adam_step(self.p, self.g, self.m, self.v, self.step_t, self.ticket,
                                  self.lr, float(self.betas[0]), float(self.betas[1]), self.eps,
                                  self.wd)
+
+
+def muon_matrices(model: torch.nn.Module, params) -> list:
+    """The parameters ``TrainStep(optimizer="muon")`` updates with Muon: the 2-D
+    ones apart from the output head's (``model.linear``)."""
+    head = getattr(model, "linear", None)
+    out = {id(p) for p in head.parameters()} if isinstance(head, torch.nn.Module) else set()
+    return [p for p in params if p.dim() == 2 and id(p) not in out]
+
+
+class FlatMuon:
+    """Muon (``muon.muon_step``) for the weight matrices and Adam for the rest, over
+    flat parameter and gradient buffers that hold the matrices last
+    (``flatten_params(rest + matrices, align=4)``).  The matrices' learning rate is
+    scaled by 0.2 sqrt(max(rows, cols)), which gives an update the root mean square of
+    an Adam step, so one ``lr`` serves both."""
+
+    ALIGN = 4  # elements: both optimisers' 16-B loads
+
+    def __init__(self, flat_params: torch.Tensor, flat_grads: torch.Tensor, rest, matrices,
+                 lr: float = 1e-3, momentum: float = 0.95, nesterov: bool = True,
+                 weight_decay: float = 0.0):
+        from .muon import muon_step
+        self._muon_step = muon_step
+        offs, _ = _offsets(list(rest) + list(matrices), self.ALIGN)
+        offs = offs[len(rest):]
+        first = offs[0] if offs else flat_params.numel()
+        if first:
+            p, g = flat_params[:first], flat_grads[:first]
+        else:  # nothing for Adam: its step count still keys the device dropout
+            p, g = flat_params.new_zeros(4), flat_grads.new_zeros(4)
+        self.adam = FlatAdam(p, g, lr)
+        self.buf = torch.zeros_like(flat_params[first:])
+        self.w, self.g, self.m = [], [], []
+        for q, off in zip(matrices, offs):
+            k = q.numel()
+            self.w.append(flat_params[off:off + k].view_as(q))
+            self.g.append(flat_grads[off:off + k].view_as(q))
+            self.m.append(self.buf[off - first:off - first + k].view_as(q))
+        self.lr, self.momentum, self.nesterov = float(lr), float(momentum), bool(nesterov)
+        self.wd = float(weight_decay)
+
+    # the matrices' gradients are cleared by the step's own fill
+    zeroes_grads = False
+
+    @property
+    def step_t(self) -> torch.Tensor:
+        return self.adam.step_t
+
+    def state(self) -> list:
+        return self.adam.state() + [self.buf]
+
+    def step(self) -> None:
+        self.adam.step()
+        self._muon_step(self.w, self.g, self.m, lr=self.lr, momentum=self.momentum,
+                        nesterov=self.nesterov, weight_decay=self.wd,
+                        adjust_lr="match_rms_adamw")
 
 
 def _host_staged(t: torch.Tensor, group) -> bool:
@@ -159,6 +230,9 @@ class TrainStep:
     Constructing it applies no update: the warm-up steps before capture are
     undone (parameters, buffers, optimizer state, RNG).
 
+    ``optimizer``: "sv2n" (Adam over the flat buffers, one launch), "muon" (Muon for
+    the weight matrices, Adam for the rest: ``FlatMuon``), else torch's Adam.
+
     ``loss_sum``: a device scalar every step adds its loss to inside the
     captured step (the reference's per-epoch running loss,
     5_train_SpotV2Net.py:160-163, without an eager launch per step)."""
@@ -175,14 +249,23 @@ class TrainStep:
         self.group = group
         self.warmup = warmup
         self.params = [p for p in model.parameters() if p.requires_grad]
-        self.flat_params = flatten_params(self.params)
-        self.flat = flatten_grads(self.params)
-        self.opt = FlatAdam(self.flat_params, self.flat, lr) if optimizer == "sv2n" \
-            else make_adam(self.params, lr)
+        if optimizer == "muon":
+            matrices = muon_matrices(model, self.params)
+            ids = {id(p) for p in matrices}
+            rest = [p for p in self.params if id(p) not in ids]
+            self.params = rest + matrices
+            self.flat_params = flatten_params(self.params, FlatMuon.ALIGN)
+            self.flat = flatten_grads(self.params, FlatMuon.ALIGN)
+            self.opt = FlatMuon(self.flat_params, self.flat, rest, matrices, lr)
+        else:
+            self.flat_params = flatten_params(self.params)
+            self.flat = flatten_grads(self.params)
+            self.opt = FlatAdam(self.flat_params, self.flat, lr) if optimizer == "sv2n" \
+                else make_adam(self.params, lr)
         # post-layer dropout uniforms keyed by (seed, Adam's device step
         # count, layer) (stack.device_dropout): no torch random op in the
         # captured step; device_rng=False keeps torch's generator
-        self.device_rng = device_rng and isinstance(self.opt, FlatAdam)
+        self.device_rng = device_rng and isinstance(self.opt, (FlatAdam, FlatMuon))
         self.dropout_seed = int(torch.initial_seed() if dropout_seed is None else dropout_seed)
         self.distributed = dist.is_available() and dist.is_initialized() and \
             dist.get_world_size(group) > 1
@@ -282,8 +365,8 @@ class TrainStep:
                 "buffers": [b.detach().clone() for b in self.model.buffers()],
                 "cpu_rng": torch.get_rng_state(),
                 "cuda_rng": torch.cuda.get_rng_state(self.flat.device)}
-        if isinstance(self.opt, FlatAdam):
-            snap["opt"] = (self.opt.m.clone(), self.opt.v.clone(), self.opt.step_t.clone())
+        if isinstance(self.opt, (FlatAdam, FlatMuon)):
+            snap["opt"] = [t.clone() for t in self.opt.state()]
         else:
             snap["opt"] = {id(p): {k: (v.clone() if torch.is_tensor(v) else v)
                                    for k, v in st.items()}
@@ -300,11 +383,9 @@ class TrainStep:
             for b, old in zip(self.model.buffers(), snap["buffers"]):
                 b.copy_(old)
             self.flat.zero_()
-            if isinstance(self.opt, FlatAdam):
-                m, v, t = snap["opt"]
-                self.opt.m.copy_(m)
-                self.opt.v.copy_(v)
-                self.opt.step_t.copy_(t)
+            if isinstance(self.opt, (FlatAdam, FlatMuon)):
+                for t, old in zip(self.opt.state(), snap["opt"]):
+                    t.copy_(old)
             else:  # torch.optim.Adam: state tensors back to their pre-warm-up values
                 for p, st in self.opt.state.items():
                     old = snap["opt"].get(id(p))
@@ -615,10 +696,11 @@ class Fit:
 def fit(model: torch.nn.Module, dataset, num_epochs: int, batch_size: int, lr: float = 1e-3,
         split: float = 0.8, generator: Optional[torch.Generator] = None, use_graph: bool = True,
         checkpoint_path: Optional[str] = None, tolerance: float = 1e-9,
-        step_hook: Optional[Callable[[int, int], None]] = None) -> list:
+        step_hook: Optional[Callable[[int, int], None]] = None, optimizer: str = "sv2n") -> list:
     """Train like 5_train_SpotV2Net.py:139-197 and return the per-epoch history
     (train/test loss and RMSE).  See ``Fit``."""
-    f = Fit(model, dataset, batch_size, lr, split, generator, use_graph, step_hook=step_hook)
+    f = Fit(model, dataset, batch_size, lr, split, generator, use_graph, optimizer,
+            step_hook=step_hook)
     for _ in range(num_epochs):
         f.run_epoch(checkpoint_path, tolerance)
     return f.history
