@@ -25,7 +25,21 @@ endif
 SRC := $(wildcard spotv2net_amd/csrc/*.hip)
 OBJ := $(patsubst spotv2net_amd/csrc/%.hip,$(BUILD)/%.o,$(SRC))
 
-all: $(LIB)
+# the operators whose host side is C++ (host code only; the C++ compiler torch's
+# headers and libraries were built for)
+TORCH_LIB ?= spotv2net_amd/libsv2n_torch.so
+PYTHON ?= python3
+TORCH_DIR = $(shell $(PYTHON) -c "import importlib.util as u; print(u.find_spec('torch').submodule_search_locations[0])")
+ROCM ?= /opt/rocm
+CXX = g++
+CXXFLAGS ?= -O2 -std=c++17 -fPIC -Wall
+
+all: $(LIB) $(TORCH_LIB)
+
+$(TORCH_LIB): spotv2net_amd/csrc/sv2n_torch.cpp include/sv2n.h
+	$(CXX) $(CXXFLAGS) -D__HIP_PLATFORM_AMD__=1 -DUSE_ROCM -Iinclude -isystem $(TORCH_DIR)/include \
+	  -isystem $(TORCH_DIR)/include/torch/csrc/api/include -isystem $(ROCM)/include -shared -o $@ $< \
+	  -L$(TORCH_DIR)/lib -ltorch -ltorch_cpu -lc10 -lc10_hip
 
 $(BUILD)/%.o: spotv2net_amd/csrc/%.hip $(wildcard spotv2net_amd/csrc/*.h) include/sv2n.h
 	@mkdir -p $(BUILD)
@@ -35,6 +49,6 @@ $(LIB): $(OBJ)
 	$(HIPCC) $(HIPFLAGS) -shared -o $@ $(OBJ)
 
 clean:
-	rm -rf build $(LIB)
+	rm -rf build $(LIB) $(TORCH_LIB)
 
 .PHONY: all clean

@@ -203,6 +203,30 @@ def load() -> ctypes.CDLL:
     return lib
 
 
+# the operators whose host side is C++ (csrc/sv2n_torch.cpp)
+TORCH_LIB_PATH = os.path.join(_HERE, "libsv2n_torch.so")
+_torch_lib = None
+
+
+def load_torch_ops() -> None:
+    """Load libsv2n_torch.so once (it registers the C++ operators on import) and
+    hand it the C entries of the loaded libsv2n; NativeLibraryError if one of the
+    two is absent or stale."""
+    global _torch_lib
+    if _torch_lib is not None:
+        return
+    lib = load()
+    if not os.path.exists(TORCH_LIB_PATH):
+        raise NativeLibraryError(f"{TORCH_LIB_PATH} not found: build it with `make`")
+    t = ctypes.CDLL(TORCH_LIB_PATH)
+    t.sv2n_torch_bind.restype = None
+    t.sv2n_torch_bind.argtypes = [_p] * 4
+    t.sv2n_torch_bind(*[ctypes.cast(getattr(lib, n), _p) for n in (
+        "sv2n_layer_norm_fwd", "sv2n_layer_norm_bwd", "sv2n_layer_norm_bwd_workspace",
+        "sv2n_strerror")])
+    _torch_lib = t
+
+
 def check(rc: int, what: str) -> None:
     if rc != 0:
         msg = load().sv2n_strerror(rc).decode()

@@ -1,0 +1,272 @@
+// The layer-norm operators' host side in C++: their kernels take a few microseconds,
+// less than an operator implemented in Python costs to call, and an autograd node in
+// Python costs more than both passes.  Registers, for the schemas library.py defines,
+//   sv2n::layer_norm          CUDA kernel and autograd formula
+//   sv2n::layer_norm_bwd      CUDA kernel
+//   sv2n::layer_norm_bwd_acc  CUDA kernel
+// The C entries come from whichever libsv2n build the process loaded: _lib.py hands
+// their addresses to sv2n_torch_bind before the first call.
+#include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/library.h>
+
+#include <optional>
+#include <tuple>
+
+#include "sv2n.h"
+
+namespace {
+
+using at::Tensor;
+using OptTensor = std::optional<Tensor>;
+
+struct Entries {
+  decltype(&sv2n_layer_norm_fwd) fwd = nullptr;
+  decltype(&sv2n_layer_norm_bwd) bwd = nullptr;
+  decltype(&sv2n_layer_norm_bwd_workspace) bwd_ws = nullptr;
+  decltype(&sv2n_strerror) strerror = nullptr;
+} g_entries;
+
+void check(int rc, const char* what) {
+  TORCH_CHECK(rc == 0, what, " failed (code ", rc, "): ", g_entries.strerror(rc));
+}
+
+int dtype_code(at::ScalarType t) {
+  switch (t) {
+    case at::kFloat: return SV2N_DT_F32;
+    case at::kBFloat16: return SV2N_DT_BF16;
+    case at::kHalf: return SV2N_DT_F16;
+    default: return -1;
+  }
+}
+
+// x as [rows, cols] with unit column stride and a row stride of at least a row: a view
+// where its strides allow one, else a dense copy
+Tensor rows_of(const Tensor& x) {
+  const int64_t cols = x.size(-1);
+  Tensor r = x.dim() == 2 ? x : x.reshape({-1, cols});
+  if ((cols > 1 && r.stride(1) != 1) || (r.size(0) > 1 && r.stride(0) < cols)) r = r.contiguous();
+  return r;
+}
+int64_t row_stride(const Tensor& r) { return r.size(0) > 1 ? r.stride(0) : r.size(1); }
+
+// Refuses what the kernels do not take; the type code of the weight
+int check_inputs(const Tensor& x, const OptTensor& weight, const OptTensor& bias) {
+  TORCH_CHECK(g_entries.fwd, "sv2n: the kernels' library is not loaded");
+  TORCH_CHECK(x.dim() >= 1, "sv2n: layer_norm: expected at least one dimension");
+  const int64_t cols = x.size(-1);
+  TORCH_CHECK(dtype_code(x.scalar_type()) >= 0,
+              "sv2n: layer_norm: expected float32, bfloat16 or float16, got ", x.scalar_type());
+  TORCH_CHECK(cols >= 1 && cols <= SV2N_LN_MAX_COLS, "sv2n: layer_norm: rows of 1 to ",
+              SV2N_LN_MAX_COLS, " elements, got ", cols);
+  std::optional<at::ScalarType> type;
+  const char* name = "weight";
+  for (const OptTensor* t : {&weight, &bias}) {
+    if (t->has_value()) {
+      const Tensor& v = **t;
+      TORCH_CHECK(v.dim() == 1 && v.size(0) == cols, "sv2n: layer_norm: ", name, " of shape ",
+                  v.sizes(), " for rows of ", cols);
+      TORCH_CHECK(v.device() == x.device(), "sv2n: layer_norm: ", name, " on ", v.device(),
+                  ", input on ", x.device());
+      TORCH_CHECK(v.scalar_type() == at::kFloat || v.scalar_type() == x.scalar_type(),
+                  "sv2n: layer_norm: ", name, " is ", v.scalar_type(),
+                  "; expected float32 or the input's ", x.scalar_type());
+      TORCH_CHECK(!type || *type == v.scalar_type(),
+                  "sv2n: layer_norm: weight and bias of different types");
+      type = v.scalar_type();
+    }
+    name = "bias";
+  }
+  return dtype_code(type.value_or(x.scalar_type()));
+}
+
+hipStream_t stream_of(const Tensor& x) {
+  return c10::hip::getCurrentHIPStream(x.device().index()).stream();
+}
+
+const void* data_of(const Tensor& t) { return t.numel() ? t.const_data_ptr() : nullptr; }
+
+std::tuple<Tensor, Tensor, Tensor> layer_norm(const Tensor& x, const OptTensor& weight,
+                                              const OptTensor& bias, double eps) {
+  const int wdt = check_inputs(x, weight, bias);
+  TORCH_CHECK(eps >= 0.0, "sv2n: layer_norm: eps must not be negative, got ", eps);
+  const c10::OptionalDeviceGuard guard(x.device());
+  const Tensor r = rows_of(x);
+  const int64_t rows = r.size(0), cols = r.size(1);
+  Tensor y = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
+  Tensor mean = at::empty({rows}, x.options().dtype(at::kFloat));
+  Tensor rstd = at::empty({rows}, x.options().dtype(at::kFloat));
+  if (rows) {
+    const Tensor w = weight ? weight->contiguous() : Tensor(), b = bias ? bias->contiguous() : Tensor();
+    check(g_entries.fwd(r.const_data_ptr(), row_stride(r), dtype_code(x.scalar_type()),
+                        w.defined() ? w.const_data_ptr() : nullptr,
+                        b.defined() ? b.const_data_ptr() : nullptr, wdt, rows, (int)cols, (float)eps,
+                        y.mutable_data_ptr(), mean.mutable_data_ptr<float>(),
+                        rstd.mutable_data_ptr<float>(), stream_of(x)),
+          "sv2n_layer_norm_fwd");
+  }
+  return {y, mean, rstd};
+}
+
+// dx (undefined unless asked for); dw and db into what is given
+Tensor backward_into(const Tensor& dy, const Tensor& x, const OptTensor& weight, const Tensor& mean,
+                     const Tensor& rstd, bool need_dx, const OptTensor& dw, const OptTensor& db,
+                     bool accumulate) {
+  int wdt = check_inputs(x, weight, std::nullopt);
+  TORCH_CHECK(dy.sizes() == x.sizes() && dy.scalar_type() == x.scalar_type() &&
+                  dy.device() == x.device(),
+              "sv2n: layer_norm_bwd: dy ", dy.sizes(), " ", dy.scalar_type(), " for x ", x.sizes(),
+              " ", x.scalar_type());
+  const c10::OptionalDeviceGuard guard(x.device());
+  const Tensor r = rows_of(x), d = rows_of(dy);
+  const int64_t rows = r.size(0), cols = r.size(1);
+  for (const Tensor* t : {&mean, &rstd})
+    TORCH_CHECK(t->scalar_type() == at::kFloat && t->numel() == rows && t->is_contiguous() &&
+                    t->device() == x.device(),
+                "sv2n: layer_norm_bwd: mean / rstd are the forward's");
+  for (const OptTensor* g : {&dw, &db}) {
+    if (!g->has_value()) continue;
+    const Tensor& v = **g;
+    TORCH_CHECK(v.dim() == 1 && v.size(0) == cols && v.is_contiguous() && v.device() == x.device() &&
+                    (v.scalar_type() == at::kFloat || v.scalar_type() == x.scalar_type()),
+                "sv2n: layer_norm_bwd: gradient buffer");
+    if (!weight) wdt = dtype_code(v.scalar_type());
+    TORCH_CHECK(dtype_code(v.scalar_type()) == wdt,
+                "sv2n: layer_norm_bwd: gradients and weight of different types");
+  }
+  Tensor dx;
+  if (need_dx) dx = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
+  const bool wg = dw.has_value() || db.has_value();
+  const int dt = dtype_code(x.scalar_type());
+  const int64_t ws_n = wg ? g_entries.bwd_ws(rows, (int)cols, dt) : 0;
+  Tensor ws;
+  if (ws_n) ws = at::empty({ws_n}, x.options().dtype(at::kFloat));
+  const Tensor w = weight ? weight->contiguous() : Tensor();
+  check(g_entries.bwd(data_of(d), row_stride(d), data_of(r), row_stride(r), dt,
+                      w.defined() ? w.const_data_ptr() : nullptr, wdt,
+                      (const float*)data_of(mean), (const float*)data_of(rstd), rows, (int)cols,
+                      dx.defined() && dx.numel() ? dx.mutable_data_ptr() : nullptr,
+                      dw ? dw->mutable_data_ptr() : nullptr, db ? db->mutable_data_ptr() : nullptr,
+                      accumulate, ws_n ? ws.mutable_data_ptr<float>() : nullptr, ws_n,
+                      stream_of(x)),
+        "sv2n_layer_norm_bwd");
+  return dx;
+}
+
+std::tuple<Tensor, Tensor, Tensor> layer_norm_bwd(const Tensor& dy, const Tensor& x,
+                                                  const OptTensor& weight, const Tensor& mean,
+                                                  const Tensor& rstd, bool need_dx, bool need_dw,
+                                                  bool need_db,
+                                                  std::optional<at::ScalarType> grad_dtype) {
+  const auto type = weight ? weight->scalar_type() : grad_dtype.value_or(x.scalar_type());
+  const auto opts = x.options().dtype(type);
+  const int64_t cols = x.dim() ? x.size(-1) : 0;
+  OptTensor dw, db;
+  if (need_dw) dw = at::empty({cols}, opts);
+  if (need_db) db = at::empty({cols}, opts);
+  Tensor dx = backward_into(dy, x, weight, mean, rstd, need_dx, dw, db, false);
+  auto or_none = [&](const Tensor& t) { return t.defined() ? t : at::empty({0}, x.options()); };
+  return {or_none(dx), or_none(dw.value_or(Tensor())), or_none(db.value_or(Tensor()))};
+}
+
+Tensor layer_norm_bwd_acc(const Tensor& dy, const Tensor& x, const OptTensor& weight,
+                          const Tensor& mean, const Tensor& rstd, const OptTensor& g_weight,
+                          const OptTensor& g_bias) {
+  return backward_into(dy, x, weight, mean, rstd, true, g_weight, g_bias, true);
+}
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+std::tuple<Tensor, Tensor, Tensor> call_layer_norm(const Tensor& x, const OptTensor& weight,
+                                                   const OptTensor& bias, double eps) {
+  static auto op = c10::Dispatcher::singleton()
+                       .findSchemaOrThrow("sv2n::layer_norm", "")
+                       .typed<decltype(layer_norm)>();
+  return op.call(x, weight, bias, eps);
+}
+std::tuple<Tensor, Tensor, Tensor> call_layer_norm_bwd(const Tensor& dy, const Tensor& x,
+                                                       const OptTensor& weight, const Tensor& mean,
+                                                       const Tensor& rstd, bool need_dx,
+                                                       bool need_dw, bool need_db,
+                                                       std::optional<at::ScalarType> grad_dtype) {
+  static auto op = c10::Dispatcher::singleton()
+                       .findSchemaOrThrow("sv2n::layer_norm_bwd", "")
+                       .typed<decltype(layer_norm_bwd)>();
+  return op.call(dy, x, weight, mean, rstd, need_dx, need_dw, need_db, grad_dtype);
+}
+
+struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptTensor& weight,
+                               const OptTensor& bias, double eps) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [y, mean, rstd] = call_layer_norm(x, weight, bias, eps);
+    ctx->save_for_backward({x, weight.value_or(Tensor()), mean, rstd});
+    ctx->saved_data["bias_type"] =
+        bias ? std::optional<int64_t>((int64_t)bias->scalar_type()) : std::nullopt;
+    ctx->mark_non_differentiable({mean, rstd});
+    return {y, mean, rstd};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
+    const bool twice = at::GradMode::is_enabled();
+    variable_list out(4);
+    {
+      at::AutoDispatchBelowAutograd below;
+      const auto saved = ctx->get_saved_variables();
+      const OptTensor weight = saved[1].defined() ? OptTensor(saved[1]) : std::nullopt;
+      const auto bt = ctx->saved_data["bias_type"].toOptional<int64_t>();
+      std::optional<at::ScalarType> type;
+      if (bt) type = (at::ScalarType)*bt;
+      // (counted over the tensors that were given)
+      const bool nx = ctx->needs_input_grad(0), nw = weight && ctx->needs_input_grad(1);
+      const bool nb = bt && ctx->needs_input_grad(weight ? 2 : 1);
+      auto [dx, dw, db] = call_layer_norm_bwd(grads[0], saved[0], weight, saved[2], saved[3], nx,
+                                              nw, nb, type);
+      if (nx) out[0] = dx;
+      if (nw) out[1] = dw;
+      if (nb) out[2] = db;
+    }
+    if (twice) {
+      // differentiable once: a gradient of these gradients raises
+      for (auto& t : out)
+        if (t.defined()) t = t.detach().requires_grad_(true);
+      auto err = std::make_shared<torch::autograd::DelayedError>(
+          "sv2n: layer_norm is differentiable once (its gradients have no gradient)", 4);
+      out = (*err)(std::move(out));
+    }
+    return out;
+  }
+};
+
+std::tuple<Tensor, Tensor, Tensor> layer_norm_autograd(const Tensor& x, const OptTensor& weight,
+                                                       const OptTensor& bias, double eps) {
+  const bool need = at::GradMode::is_enabled() &&
+                    (x.requires_grad() || (weight && weight->requires_grad()) ||
+                     (bias && bias->requires_grad()));
+  if (!need) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return call_layer_norm(x, weight, bias, eps);
+  }
+  auto out = LayerNormFn::apply(x, weight, bias, eps);
+  return {out[0], out[1], out[2]};
+}
+
+}  // namespace
+
+TORCH_LIBRARY_IMPL(sv2n, CUDA, m) {
+  m.impl("layer_norm", layer_norm);
+  m.impl("layer_norm_bwd", layer_norm_bwd);
+  m.impl("layer_norm_bwd_acc", layer_norm_bwd_acc);
+}
+TORCH_LIBRARY_IMPL(sv2n, Autograd, m) { m.impl("layer_norm", layer_norm_autograd); }
+
+extern "C" void sv2n_torch_bind(void* fwd, void* bwd, void* bwd_ws, void* strerror) {
+  g_entries.fwd = (decltype(g_entries.fwd))fwd;
+  g_entries.bwd = (decltype(g_entries.bwd))bwd;
+  g_entries.bwd_ws = (decltype(g_entries.bwd_ws))bwd_ws;
+  g_entries.strerror = (decltype(g_entries.strerror))strerror;
+}

@@ -1275,41 +1275,7 @@ def _project_a16_fake(a_bf16, k, planes, w):
 OPS = tuple(_SCHEMAS)
 
 
-# --------------------------------------------------------------------------
-# layer norm (sv2n_layer_norm_fwd / _bwd)
-# --------------------------------------------------------------------------
 _DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # SV2N_DT_*
-LN_MAX_COLS = 16384  # SV2N_LN_MAX_COLS
-
-
-def _ln_rows(x: torch.Tensor) -> torch.Tensor:
-    """``x`` as [rows, cols] with unit column stride and a row stride of at
-    least a row: a view where its strides allow one, else a dense copy."""
-    if x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= x.shape[1]:
-        return x
-    x = x.reshape(-1, x.shape[-1])
-    if (x.stride(1) != 1 and x.shape[1] > 1) or (x.stride(0) < x.shape[1] and x.shape[0] > 1):
-        x = x.contiguous()
-    return x
-
-
-def _ln_check(x, weight, bias) -> int:
-    """Refuses what the kernels do not take; the code of the weight's type."""
-    _need(x.dim() >= 1, "layer_norm: expected at least one dimension")
-    cols = x.shape[-1]
-    _need(x.dtype in _DT, f"layer_norm: expected float32, bfloat16 or float16, got {x.dtype}")
-    _need(1 <= cols <= LN_MAX_COLS, f"layer_norm: rows of 1 to {LN_MAX_COLS} elements, got {cols}")
-    wdt = None
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is None:
-            continue
-        _need(t.shape == (cols,), f"layer_norm: {name} of shape {tuple(t.shape)} for rows of {cols}")
-        _need(t.device == x.device, f"layer_norm: {name} on {t.device}, input on {x.device}")
-        _need(t.dtype in (torch.float32, x.dtype),
-              f"layer_norm: {name} is {t.dtype}; expected float32 or the input's {x.dtype}")
-        _need(wdt in (None, t.dtype), "layer_norm: weight and bias of different types")
-        wdt = t.dtype
-    return _DT[wdt if wdt is not None else x.dtype]
 
 
 class _on_device:
@@ -1331,26 +1297,18 @@ class _on_device:
             torch.cuda.set_device(self.old)
 
 
-def _vec(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    return None if t is None else t.contiguous()
+# --------------------------------------------------------------------------
+# layer norm (sv2n_layer_norm_fwd / _bwd): implemented, with its autograd formula,
+# in csrc/sv2n_torch.cpp
+# --------------------------------------------------------------------------
+try:
+    _lib.load_torch_ops()
+except (_lib.NativeLibraryError, AttributeError, OSError) as _err:  # not built: the calls say so
+    def _not_built(*args, _msg=str(_err), **kwargs):
+        raise _lib.NativeLibraryError("sv2n layer norm: " + _msg)
 
-
-@_impl("layer_norm")
-def _layer_norm(x, weight, bias, eps):
-    wdt = _ln_check(x, weight, bias)
-    _need(eps >= 0.0, f"layer_norm: eps must not be negative, got {eps}")
-    x2, weight, bias = _ln_rows(x), _vec(weight), _vec(bias)
-    rows, cols = x2.shape
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    mean = torch.empty(rows, device=x.device, dtype=torch.float32)
-    rstd = torch.empty(rows, device=x.device, dtype=torch.float32)
-    if rows:
-        with _on_device(x):
-            _lib.check(_lib.load().sv2n_layer_norm_fwd(
-                x2.data_ptr(), x2.stride(0) if rows > 1 else cols, _DT[x.dtype], _lib.ptr(weight),
-                _lib.ptr(bias), wdt, rows, cols, eps, y.data_ptr(), mean.data_ptr(),
-                rstd.data_ptr(), _st(x)), "sv2n_layer_norm_fwd")
-    return y, mean, rstd
+    for _name in ("layer_norm", "layer_norm_bwd", "layer_norm_bwd_acc"):
+        LIB.impl(_name, _not_built, "CUDA")
 
 
 @_fake("layer_norm")
@@ -1360,66 +1318,13 @@ def _layer_norm_fake(x, weight, bias, eps):
             x.new_empty(rows, dtype=torch.float32), x.new_empty(rows, dtype=torch.float32))
 
 
-def _ln_bwd(dy, x, weight, mean, rstd, need_dx, dw, db, accumulate):
-    wdt = _ln_check(x, weight, None)
-    _need(dy.shape == x.shape and dy.dtype == x.dtype and dy.device == x.device,
-          f"layer_norm_bwd: dy {tuple(dy.shape)} {dy.dtype} for x {tuple(x.shape)} {x.dtype}")
-    x2, dy2, weight = _ln_rows(x), _ln_rows(dy), _vec(weight)
-    rows, cols = x2.shape
-    for t in (mean, rstd):
-        _need(t.dtype == torch.float32 and t.numel() == rows and t.is_contiguous() and
-              t.device == x.device, "layer_norm_bwd: mean / rstd are the forward's")
-    for g in (dw, db):
-        if g is None:
-            continue
-        _need(g.shape == (cols,) and g.is_contiguous() and g.device == x.device and
-              g.dtype in (torch.float32, x.dtype), "layer_norm_bwd: gradient buffer")
-        if weight is None:
-            wdt = _DT[g.dtype]
-        _need(_DT[g.dtype] == wdt, "layer_norm_bwd: gradients and weight of different types")
-    dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need_dx else None
-    lib = _lib.load()
-    wg = dw is not None or db is not None
-    ws_n = lib.sv2n_layer_norm_bwd_workspace(rows, cols, _DT[x.dtype]) if wg else 0
-    ws = torch.empty(ws_n, device=x.device, dtype=torch.float32) if ws_n else None
-    with _on_device(x):
-        _lib.check(lib.sv2n_layer_norm_bwd(
-            _p(dy2), dy2.stride(0) if rows > 1 else cols, _p(x2),
-            x2.stride(0) if rows > 1 else cols, _DT[x.dtype], _lib.ptr(weight), wdt, _p(mean),
-            _p(rstd), rows, cols, None if dx is None else _p(dx), _lib.ptr(dw), _lib.ptr(db),
-            int(accumulate), _lib.ptr(ws), ws_n, _st(x)), "sv2n_layer_norm_bwd")
-    return dx
-
-
-def _ln_grad_dtype(x, weight, grad_dtype):
-    """The type of dw and db: the weight's, or (without one) the asked type."""
-    if weight is not None:
-        return weight.dtype
-    return x.dtype if grad_dtype is None else grad_dtype
-
-
-@_impl("layer_norm_bwd")
-def _layer_norm_bwd(dy, x, weight, mean, rstd, need_dx, need_dw, need_db, grad_dtype=None):
-    cols = x.shape[-1]
-    dt = _ln_grad_dtype(x, weight, grad_dtype)
-    dw = torch.empty(cols, device=x.device, dtype=dt) if need_dw else None
-    db = torch.empty(cols, device=x.device, dtype=dt) if need_db else None
-    dx = _ln_bwd(dy, x, weight, mean, rstd, need_dx, dw, db, False)
-    return tuple(t if t is not None else x.new_empty(0) for t in (dx, dw, db))
-
-
 @_fake("layer_norm_bwd")
 def _layer_norm_bwd_fake(dy, x, weight, mean, rstd, need_dx, need_dw, need_db, grad_dtype=None):
     cols = x.shape[-1]
-    dt = _ln_grad_dtype(x, weight, grad_dtype)
+    dt = weight.dtype if weight is not None else x.dtype if grad_dtype is None else grad_dtype
     return (torch.empty(x.shape if need_dx else (0,), device=x.device, dtype=x.dtype),
             x.new_empty(cols, dtype=dt) if need_dw else x.new_empty(0),
             x.new_empty(cols, dtype=dt) if need_db else x.new_empty(0))
-
-
-@_impl("layer_norm_bwd_acc")
-def _layer_norm_bwd_acc(dy, x, weight, mean, rstd, g_weight, g_bias):
-    return _ln_bwd(dy, x, weight, mean, rstd, True, g_weight, g_bias, True)
 
 
 @_fake("layer_norm_bwd_acc")

@@ -13,27 +13,8 @@ from typing import Optional
 
 import torch
 from torch import nn
-from torch.autograd.function import once_differentiable
 
 from . import library  # noqa: F401  (registers torch.ops.sv2n.layer_norm)
-
-
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        y, mean, rstd = torch.ops.sv2n.layer_norm(x, weight, bias, eps)
-        ctx.bias_dtype = None if bias is None else bias.dtype
-        ctx.save_for_backward(x, weight, mean, rstd)
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, weight, mean, rstd = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dx, dw, db = torch.ops.sv2n.layer_norm_bwd(dy, x, weight, mean, rstd, need[0], need[1],
-                                                   need[2], ctx.bias_dtype)
-        return dx if need[0] else None, dw if need[1] else None, db if need[2] else None, None
 
 
 def _check_device(x: torch.Tensor) -> None:
@@ -48,10 +29,6 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     (biased variance); differentiable once in x, weight and bias.  The result is
     dense and of x's type."""
     _check_device(x)
-    if torch.is_grad_enabled() and (x.requires_grad or
-                                    (weight is not None and weight.requires_grad) or
-                                    (bias is not None and bias.requires_grad)):
-        return _LayerNorm.apply(x, weight, bias, eps)
     return torch.ops.sv2n.layer_norm(x, weight, bias, eps)[0]
 
 

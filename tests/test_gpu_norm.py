@@ -319,3 +319,19 @@ def test_opcheck(dev):
     gw = torch.zeros(100, device=dev)
     torch.library.opcheck(ops.layer_norm_bwd_acc, (dy, x, w, mean, rstd, gw, None),
                           test_utils=utils)
+
+
+def test_compiles(dev):
+    """torch.compile traces the operator and its autograd formula."""
+    from spotv2net_amd import layer_norm
+    x, w, b, dy = make(dev, 50, 120, torch.float32, torch.float32)
+    want = run(x, w, b, dy)
+
+    def f(x, w, b):
+        return layer_norm(x * 1.0, w, b) * 1.0
+
+    xs = [t.detach().requires_grad_() for t in (x, w, b)]
+    y = torch.compile(f, backend="aot_eager")(*xs)
+    got = (y.detach(),) + torch.autograd.grad(y, xs, dy)
+    for a, r in zip(got, want):
+        assert torch.equal(a, r)

@@ -195,7 +195,7 @@ def test_training_steps_match_restatement(dev, use_graph):
         opt.step()
         got = step()
         torch.cuda.synchronize()
-        assert abs(float(got) - float(loss)) <= (1e-5 if k == 0 else 1e-3) * max(1.0, float(loss)), k
+        assert abs(float(got) - float(loss.detach())) <= (1e-5 if k == 0 else 1e-3) * max(1.0, float(loss.detach())), k
         if k == 0:
             for name, p, q in named(model, ref):
                 if p.dim() == 2 and "linear" not in name:   # U to f32 accuracy, times lr
