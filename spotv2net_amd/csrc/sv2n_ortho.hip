@@ -14,6 +14,10 @@
 // 64 bits the result is as close as one of f32 products (the steps amplify any
 // rounding of the input by up to a^steps, so fewer bits are not enough for f32).
 //
+// (Where the smaller side is at most 32 the sums are so short that those 22 bits would
+// be the largest error, up to 3.6 times that of f32 products; the work there is next to
+// nothing, so the operands are f32 and the products v_mfma_f32_32x32x2_f32.)
+//
 // S and S S are symmetric: only tiles on and below the diagonal are computed and
 // each is stored twice.  Every operand is stored with its K dimension contiguous
 // (X for S, Xt for Q X), so one kernel with one staging scheme serves all three
@@ -42,6 +46,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 constexpr int NS_MAX = 16;      // matrices of one launch
 constexpr int NS_PARTS = 1024;  // most partial sums of squares of one matrix
 constexpr int NS_PART_ELEMS = 4096;
+constexpr int NS_EXACT = 32;    // smaller sides up to which the products are f32
 constexpr int NS_HALF = 128;    // tiles of 128 that are worth a round of their own
 constexpr int NS_TINY = 72;     // tiles of 64 below which tiles of 32 are faster
 
@@ -54,6 +59,7 @@ struct NsMat {
   int m, n, mp, np;     // m <= n, padded to the tile
   int batch, flip;      // flip: X = Gt
   int dtype;
+  int exact;            // f32 operands and products (m <= NS_EXACT)
   int parts, part_elems; // partial sums of squares per matrix, elements of each
   float lr;             // the update's factor (with buf)
   _Float16 *x, *xt[2], *s, *q;
@@ -150,9 +156,32 @@ __global__ __launch_bounds__(256) void k_ns_norm(NsArgs A, NsScale sc) {
   if (threadIdx.x == 0) M.part[(int64_t)b * M.parts + p] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-__device__ __forceinline__ void ns_split(float v, _Float16& hi, _Float16& lo) {
-  hi = (_Float16)v;
-  lo = (_Float16)(v - (float)hi);
+// A lane's 8 values of a fragment block as they are stored, and back: the hi and lo f16
+// planes, or (exact) the first and the last four as f32
+__device__ __forceinline__ void ns_pack(const float (&v)[8], bool exact, f16x8& hi, f16x8& lo) {
+  if (exact) {
+    hi = __builtin_bit_cast(f16x8, f32x4{v[0], v[1], v[2], v[3]});
+    lo = __builtin_bit_cast(f16x8, f32x4{v[4], v[5], v[6], v[7]});
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      hi[e] = (_Float16)v[e];
+      lo[e] = (_Float16)(v[e] - (float)hi[e]);
+    }
+  }
+}
+__device__ __forceinline__ void ns_unpack(f16x8 hi, f16x8 lo, bool exact, float (&v)[8]) {
+  if (exact) {
+    const f32x4 a = __builtin_bit_cast(f32x4, hi), b = __builtin_bit_cast(f32x4, lo);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[e] = a[e];
+      v[4 + e] = b[e];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (float)hi[e] + (float)lo[e];
+  }
 }
 
 // ---- 2: X_0 and its transpose as planes, one 64 x 64 tile per block ----
@@ -215,14 +244,13 @@ __global__ __launch_bounds__(256) void k_ns_split(NsArgs A, NsScale sc) {
     const int rg = (u >> 2) & 1, kg = u & 3;
     const int row = rg * 32 + (lane & 31);
     f16x8 hi, lo;
+    float f[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int k = kg * 16 + ns_k(lane >> 5, e);
-      _Float16 h, l;
-      ns_split(tr ? tile[k][row] : tile[row][k], h, l);
-      hi[e] = h;
-      lo[e] = l;
+      f[e] = tr ? tile[k][row] : tile[row][k];
     }
+    ns_pack(f, M.exact, hi, lo);
     _Float16* o = tr ? XT + ns_blk(j0 / 32 + rg, i0 / 16 + kg, M.mp)
                      : X + ns_blk(i0 / 32 + rg, j0 / 16 + kg, M.np);
     *(f16x8*)(o + lane * 8) = hi;
@@ -279,17 +307,16 @@ __device__ __forceinline__ void ns_epilogue(const f32x16& d, const NsOut& o, con
   float v[16];
 #pragma unroll
   for (int g = 0; g < 2; ++g) {
-    f16x8 ph, pl;
+    float old[8];
     if (EPI != NS_S) {
       // the old S or X at [i][j]: R's fragment of row j (S is symmetric, R = Xt)
       const _Float16* p = R + ns_blk(jb >> 5, (ib >> 4) + g, M.mp) + lane * 8;
-      ph = *(const f16x8*)p;
-      pl = *(const f16x8*)(p + 512);
+      ns_unpack(*(const f16x8*)p, *(const f16x8*)(p + 512), M.exact, old);
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       float x = d[g * 8 + e] * o.up;
-      if (EPI != NS_S) x = fmaf(o.old, (float)ph[e] + (float)pl[e], x);
+      if (EPI != NS_S) x = fmaf(o.old, old[e], x);
       v[g * 8 + e] = x;
     }
   }
@@ -333,13 +360,10 @@ __device__ __forceinline__ void ns_epilogue(const f32x16& d, const NsOut& o, con
 #pragma unroll
   for (int g = 0; g < 2; ++g) {
     f16x8 hi, lo;
+    float f[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      _Float16 a, b;
-      ns_split(v[g * 8 + e], a, b);
-      hi[e] = a;
-      lo[e] = b;
-    }
+    for (int e = 0; e < 8; ++e) f[e] = v[g * 8 + e];
+    ns_pack(f, M.exact, hi, lo);
     _Float16* p = T + ns_blk(jb >> 5, (ib >> 4) + g, M.mp) + lane * 8;
     *(f16x8*)p = hi;
     *(f16x8*)(p + 512) = lo;
@@ -354,13 +378,10 @@ __device__ __forceinline__ void ns_epilogue(const f32x16& d, const NsOut& o, con
 #pragma unroll
   for (int g = 0; g < 2; ++g) {
     f16x8 hi, lo;
+    float f[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      _Float16 a, b;
-      ns_split(tile[jl * 33 + 16 * g + ns_k(h, e)], a, b);
-      hi[e] = a;
-      lo[e] = b;
-    }
+    for (int e = 0; e < 8; ++e) f[e] = tile[jl * 33 + 16 * g + ns_k(h, e)];
+    ns_pack(f, M.exact, hi, lo);
     _Float16* p = D + ns_blk(ib >> 5, (jb >> 4) + g, kd) + lane * 8;
     *(f16x8*)p = hi;
     *(f16x8*)(p + 512) = lo;
@@ -409,6 +430,17 @@ __device__ __forceinline__ NsTile ns_tile_of(const NsArgs& A, int b) {
   }
   r.M = &M;
   return r;
+}
+
+// The eight f32 products of a pair of exact fragments: instruction q takes every lane's
+// value q, so lane half h's K values 4h + .. of both operands meet
+__device__ __forceinline__ f32x16 ns_mfma_exact(const f16x8* a, const f16x8* b, f32x16 c) {
+#pragma unroll
+  for (int q = 0; q < 8; ++q)
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(__builtin_bit_cast(f32x4, a[q >> 2])[q & 3],
+                                             __builtin_bit_cast(f32x4, b[q >> 2])[q & 3], c, 0, 0,
+                                             0);
+  return c;
 }
 
 // The three (or, PR = 1, one) f16 products of a pair of fragments
@@ -486,31 +518,40 @@ __global__ __launch_bounds__(64 * W, FT == 4 ? 1 : 2) void k_ns_mm(NsArgs A, NsS
         b[d][x][p] = *(const f16x8*)(gr + x * rg + (int64_t)k * 1024 + p * 512);
       }
   };
-  auto mul = [&](int d) {
-#pragma unroll
-    for (int x = 0; x < FT; ++x)
-#pragma unroll
-      for (int y = 0; y < FT; ++y) acc[x][y] = ns_mfma<PR>(a[d][x], b[d][y], acc[x][y]);
-  };
   // loads past the operand's end read its last block again (not used): without a
   // branch the waits count the loads in flight
+  auto run = [&](auto product) {
+    auto mul = [&](int d) {
 #pragma unroll
-  for (int d = 0; d < DEPTH; ++d) fetch(d, min(wave + d * W, nk - 1));
-  int k = wave;
-  for (; k + (DEPTH - 1) * W < nk; k += DEPTH * W) {
+      for (int x = 0; x < FT; ++x)
 #pragma unroll
-    for (int d = 0; d < DEPTH; ++d) {
-      // (the scheduler would sink the loads to their use, and the distance with them)
-      __builtin_amdgcn_sched_barrier(0);
-      mul(d);
-      __builtin_amdgcn_sched_barrier(0);
-      fetch(d, min(k + (d + DEPTH) * W, nk - 1));
+        for (int y = 0; y < FT; ++y) acc[x][y] = product(a[d][x], b[d][y], acc[x][y]);
+    };
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) fetch(d, min(wave + d * W, nk - 1));
+    int k = wave;
+    for (; k + (DEPTH - 1) * W < nk; k += DEPTH * W) {
+#pragma unroll
+      for (int d = 0; d < DEPTH; ++d) {
+        // (the scheduler would sink the loads to their use, and the distance with them)
+        __builtin_amdgcn_sched_barrier(0);
+        mul(d);
+        __builtin_amdgcn_sched_barrier(0);
+        fetch(d, min(k + (d + DEPTH) * W, nk - 1));
+      }
     }
-  }
-  __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-  for (int d = 0; d < DEPTH - 1; ++d)
-    if (k + d * W < nk) mul(d);
+    for (int d = 0; d < DEPTH - 1; ++d)
+      if (k + d * W < nk) mul(d);
+  };
+  auto f16 = [](const f16x8* p, const f16x8* q, f32x16 c) { return ns_mfma<PR>(p, q, c); };
+  if constexpr (FT == 1 && PR == 3) {
+    if (M.exact) run([](const f16x8* p, const f16x8* q, f32x16 c) { return ns_mfma_exact(p, q, c); });
+    else run(f16);
+  } else {
+    run(f16);  // (exact matrices come on FT = 1 alone)
+  }
   if constexpr (FT == 4) {
     // wave w finishes the 64 x 64 quadrant (w / 2, w % 2); two quadrants' sums at a
     // time fit the LDS
@@ -652,6 +693,7 @@ static void ns_shape(NsMat* M) {
   M->flip = M->rows > M->cols;
   M->m = std::min(M->rows, M->cols);
   M->n = std::max(M->rows, M->cols);
+  M->exact = M->m <= NS_EXACT;
   const int64_t total = (int64_t)M->rows * M->cols;
   const int64_t each = std::max<int64_t>(NS_PART_ELEMS, (total + NS_PARTS - 1) / NS_PARTS);
   M->part_elems = (int)ns_up(each, 8);
@@ -705,11 +747,12 @@ static int64_t ns_blocks(NsArgs& A, F&& per) {
   return n;
 }
 
-template <int EPI>
-static int64_t ns_count(NsArgs& A, int tile) {
+// Tiles of a product over the group's matrices that `takes` chooses
+template <int EPI, typename F>
+static int64_t ns_count(NsArgs& A, int tile, F&& takes) {
   return ns_blocks(A, [&](const NsMat& M) -> int64_t {
     const int64_t tm = M.mp / tile, tn = M.np / tile;
-    return EPI == NS_S || EPI == NS_Q ? tm * (tm + 1) / 2 : tm * tn;
+    return !takes(M) ? 0 : EPI == NS_S || EPI == NS_Q ? tm * (tm + 1) / 2 : tm * tn;
   });
 }
 
@@ -726,22 +769,30 @@ static void ns_launch(NsArgs& A, const NsScale& sc, int cur, int64_t blocks, int
 // A product over the group's tiles.  Tiles of 128 where they fill at least half of the
 // chip's 256 CUs (one block each) in every round; fewer than that left over go on
 // tiles of 64, as do products that never have so many; tiles of 32 where even those
-// are under NS_TINY (the measured sides: k_ns_mm).
+// are under NS_TINY (the measured sides: k_ns_mm).  Exact matrices run on tiles of 32,
+// in a launch of their own where the others have larger ones.
 template <int EPI, int PR>
 static void ns_product(NsArgs& A, const NsScale& sc, int cur, int pad, hipStream_t stream) {
+  auto all = [](const NsMat&) { return true; };
+  auto exact = [](const NsMat& M) { return M.exact != 0; };
+  auto split = [](const NsMat& M) { return M.exact == 0; };
+  if (ns_count<EPI>(A, 64, split) < NS_TINY) {
+    ns_launch<EPI, 1, 8, PR>(A, sc, cur, ns_count<EPI>(A, 32, all), -1, stream);
+    return;
+  }
+  int64_t big = 0;
   if (pad == 128) {
-    const int64_t n = ns_count<EPI>(A, 128);
-    int64_t big = n / 256 * 256;
+    const int64_t n = ns_count<EPI>(A, 128, split);
+    big = n / 256 * 256;
     if (n - big >= NS_HALF) big = n;
     if (big > 0) {
       ns_launch<EPI, 4, 4, PR>(A, sc, cur, big, -1, stream);
       if (n > big) ns_launch<EPI, 2, 4, PR>(A, sc, cur, 4 * (n - big), (int)big, stream);
-      return;
     }
   }
-  const int64_t n = ns_count<EPI>(A, 64);
-  if (n >= NS_TINY) ns_launch<EPI, 2, 4, PR>(A, sc, cur, n, -1, stream);
-  else ns_launch<EPI, 1, 8, PR>(A, sc, cur, ns_count<EPI>(A, 32), -1, stream);
+  if (big == 0) ns_launch<EPI, 2, 4, PR>(A, sc, cur, ns_count<EPI>(A, 64, split), -1, stream);
+  const int64_t small = ns_count<EPI>(A, 32, exact);
+  if (small > 0) ns_launch<EPI, 1, 8, PR>(A, sc, cur, small, -1, stream);
 }
 
 template <int PR>

@@ -261,7 +261,8 @@ def matrices(dev, shapes, seed=0):
 
 MODELS = [[(8, 8)], [(1, 1)], [(1, 5), (5, 1)], [(400, 1260), (400, 126), (200, 400), (200, 126)],
           [(128, 1024), (128, 12), (128, 128), (128, 12), (128, 128), (128, 12)],
-          [(33, 65)] * 16, [(20 + k, 60 - k) for k in range(35)], [(900, 1500), (3, 2)]]
+          [(33, 65)] * 16, [(700, 900), (5, 3000), (900, 31), (32, 32)],
+          [(1500, 1600), (3, 1600), (1600, 40), (2000, 1)], [(20 + k, 60 - k) for k in range(35)], [(900, 1500), (3, 2)]]
 
 
 @pytest.mark.parametrize("shapes", MODELS, ids=lambda s: f"{len(s)}x{s[0][0]}x{s[0][1]}")
