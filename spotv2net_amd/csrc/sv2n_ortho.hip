@@ -473,12 +473,12 @@ __device__ __forceinline__ f32x16 ns_mfma(const f16x8* a, const f16x8* b, f32x16
 // from big0 on, what whole rounds of FT = 4 left.
 template <int EPI, int FT, int W, int PR>
 __global__ __launch_bounds__(64 * W, FT == 4 ? 1 : 2) void k_ns_mm(NsArgs A, NsScale sc, int cur, int big0) {
-  constexpr int DEPTH = FT == 4 ? (PR == 3 ? 2 : 4) : FT == 2 ? 3 : 5;
+  // (deeper does not help: 2 to 5 steps measure the same, what bounds FT = 1 and 2 is how
+  // many lines a CU can have on the way from the L2)
+  constexpr int DEPTH = FT == 4 ? (PR == 3 ? 2 : 4) : FT == 2 ? 2 : 4;
   constexpr int PL = PR == 3 ? 2 : 1;
   constexpr int TB = 32 * FT;
-  // [place][wave][element][lane]; FT = 4: [owner of 2][wave][tile of 4][element][lane]
   extern __shared__ float s_sum[];
-  auto sum = (float (*)[W][16][64])s_sum;
   const int bx = ns_xcd(blockIdx.x, gridDim.x);
   NsTile tl;
   if (FT == 2 && big0 >= 0) {
@@ -589,28 +589,38 @@ __global__ __launch_bounds__(64 * W, FT == 4 ? 1 : 2) void k_ns_mm(NsArgs A, NsS
                        EPI == NS_X || tl.ti != tl.tj, tile);
     return;
   } else {
-#pragma unroll
-  for (int x = 0; x < FT; ++x)
-#pragma unroll
-    for (int y = 0; y < FT; ++y)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) sum[x * FT + y][wave][e][lane] = acc[x][y][e];
-  __syncthreads();
   f32x16 d;
   float* tile;
   int x = 0, y = 0;
   if constexpr (FT == 2) {
-    // wave w finishes the tile at (w / 2, w % 2)
+    // wave w finishes the tile at (w / 2, w % 2); two places' sums at a time in the LDS,
+    // so that three blocks share a CU
     static_assert(W == 4, "one wave per place");
+    auto sum = (float (*)[W][16][64])s_sum;  // [place of 2][wave][element][lane]
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (h) __syncthreads();
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sum[q][wave][e][lane] = acc[h][q][e];
+      __syncthreads();
+      if ((wave >> 1) == h) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          d[e] = (sum[wave & 1][0][e][lane] + sum[wave & 1][1][e][lane]) +
+                 (sum[wave & 1][2][e][lane] + sum[wave & 1][3][e][lane]);
+      }
+    }
     x = wave >> 1;
     y = wave & 1;
-#pragma unroll
-    for (int e = 0; e < 16; ++e)
-      d[e] = (sum[wave][0][e][lane] + sum[wave][1][e][lane]) +
-             (sum[wave][2][e][lane] + sum[wave][3][e][lane]);
-    ns_wave_sync();
-    tile = &sum[wave][0][0][0];
+    __syncthreads();
+    tile = s_sum + wave * 32 * 33;
   } else {
+    auto sum = (float (*)[W][16][64])s_sum;  // [0][wave][element][lane]
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sum[0][wave][e][lane] = acc[0][0][e];
+    __syncthreads();
     // the waves add 16 / W elements each, the first one finishes the tile
     constexpr int EW = 16 / W;
     float part[EW];
@@ -759,7 +769,7 @@ static int64_t ns_count(NsArgs& A, int tile, F&& takes) {
 template <int EPI, int FT, int W, int PR>
 static void ns_launch(NsArgs& A, const NsScale& sc, int cur, int64_t blocks, int big0,
                       hipStream_t stream) {
-  constexpr int lds = FT == 4 ? 131072 : FT * FT * W * 4096;
+  constexpr int lds = FT == 4 ? 131072 : FT == 2 ? 32768 : W * 4096;
   auto* k = k_ns_mm<EPI, FT, W, PR>;
   if (lds > 65536)
     (void)hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, lds);

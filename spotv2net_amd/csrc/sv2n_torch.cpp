@@ -9,8 +9,10 @@
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
-#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/library.h>
 
 #include <optional>
@@ -178,7 +180,7 @@ Tensor layer_norm_bwd_acc(const Tensor& dy, const Tensor& x, const OptTensor& we
   return backward_into(dy, x, weight, mean, rstd, true, g_weight, g_bias, true);
 }
 
-using torch::autograd::AutogradContext;
+using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 
 std::tuple<Tensor, Tensor, Tensor> call_layer_norm(const Tensor& x, const OptTensor& weight,
@@ -199,46 +201,47 @@ std::tuple<Tensor, Tensor, Tensor> call_layer_norm_bwd(const Tensor& dy, const T
   return op.call(dy, x, weight, mean, rstd, need_dx, need_dw, need_db, grad_dtype);
 }
 
-struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
-  static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptTensor& weight,
-                               const OptTensor& bias, double eps) {
-    at::AutoDispatchBelowADInplaceOrView below;
-    auto [y, mean, rstd] = call_layer_norm(x, weight, bias, eps);
-    ctx->save_for_backward({x, weight.value_or(Tensor()), mean, rstd});
-    ctx->saved_data["bias_type"] =
-        bias ? std::optional<int64_t>((int64_t)bias->scalar_type()) : std::nullopt;
-    ctx->mark_non_differentiable({mean, rstd});
-    return {y, mean, rstd};
-  }
-  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
-    if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
+// The backward's node.  (A Node of its own rather than a custom Function: the wrapping a
+// Function does around both passes costs more than the kernels of a small call.)
+struct LayerNormBackward : torch::autograd::Node {
+  SavedVariable x, weight, mean, rstd;
+  bool has_weight = false, has_bias = false;
+  at::ScalarType bias_type = at::kFloat;
+  bool released = false;
+
+  std::string name() const override { return "LayerNormBackward"; }
+
+  variable_list apply(variable_list&& grads) override {
+    variable_list out(3);
+    if (!grads[0].defined()) return out;
+    TORCH_CHECK(!released, torch::autograd::ERR_BACKWARD_TWICE);
     const bool twice = at::GradMode::is_enabled();
-    variable_list out(4);
     {
       at::AutoDispatchBelowAutograd below;
-      const auto saved = ctx->get_saved_variables();
-      const OptTensor weight = saved[1].defined() ? OptTensor(saved[1]) : std::nullopt;
-      const auto bt = ctx->saved_data["bias_type"].toOptional<int64_t>();
-      std::optional<at::ScalarType> type;
-      if (bt) type = (at::ScalarType)*bt;
-      // (counted over the tensors that were given)
-      const bool nx = ctx->needs_input_grad(0), nw = weight && ctx->needs_input_grad(1);
-      const bool nb = bt && ctx->needs_input_grad(weight ? 2 : 1);
-      auto [dx, dw, db] = call_layer_norm_bwd(grads[0], saved[0], weight, saved[2], saved[3], nx,
-                                              nw, nb, type);
-      if (nx) out[0] = dx;
-      if (nw) out[1] = dw;
-      if (nb) out[2] = db;
+      const OptTensor w = has_weight ? OptTensor(weight.unpack()) : std::nullopt;
+      const bool nx = task_should_compute_output(0);
+      const bool nw = has_weight && task_should_compute_output(1);
+      const bool nb = has_bias && task_should_compute_output(2);
+      auto [dx, dw, db] = call_layer_norm_bwd(
+          grads[0], x.unpack(), w, mean.unpack(), rstd.unpack(), nx, nw, nb,
+          has_bias ? std::optional<at::ScalarType>(bias_type) : std::nullopt);
+      if (nx) out[0] = std::move(dx);
+      if (nw) out[1] = std::move(dw);
+      if (nb) out[2] = std::move(db);
     }
     if (twice) {
       // differentiable once: a gradient of these gradients raises
       for (auto& t : out)
         if (t.defined()) t = t.detach().requires_grad_(true);
       auto err = std::make_shared<torch::autograd::DelayedError>(
-          "sv2n: layer_norm is differentiable once (its gradients have no gradient)", 4);
+          "sv2n: layer_norm is differentiable once (its gradients have no gradient)", 3);
       out = (*err)(std::move(out));
     }
     return out;
+  }
+  void release_variables() override {
+    released = true;
+    for (SavedVariable* v : {&x, &weight, &mean, &rstd}) v->reset_data();
   }
 };
 
@@ -247,12 +250,24 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_autograd(const Tensor& x, const Op
   const bool need = at::GradMode::is_enabled() &&
                     (x.requires_grad() || (weight && weight->requires_grad()) ||
                      (bias && bias->requires_grad()));
-  if (!need) {
+  std::tuple<Tensor, Tensor, Tensor> out;
+  {
     at::AutoDispatchBelowADInplaceOrView below;
-    return call_layer_norm(x, weight, bias, eps);
+    out = call_layer_norm(x, weight, bias, eps);
   }
-  auto out = LayerNormFn::apply(x, weight, bias, eps);
-  return {out[0], out[1], out[2]};
+  if (!need) return out;
+  std::shared_ptr<LayerNormBackward> node(new LayerNormBackward(), torch::autograd::deleteNode);
+  const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
+  node->set_next_edges(torch::autograd::collect_next_edges(x, w, b));
+  node->x = SavedVariable(x, false);
+  node->has_weight = w.defined();
+  if (node->has_weight) node->weight = SavedVariable(w, false);
+  node->has_bias = b.defined();
+  if (node->has_bias) node->bias_type = b.scalar_type();
+  node->mean = SavedVariable(std::get<1>(out), false);
+  node->rstd = SavedVariable(std::get<2>(out), false);
+  torch::autograd::set_history(std::get<0>(out), node);
+  return out;
 }
 
 }  // namespace

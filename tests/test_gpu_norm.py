@@ -335,3 +335,22 @@ def test_compiles(dev):
     got = (y.detach(),) + torch.autograd.grad(y, xs, dy)
     for a, r in zip(got, want):
         assert torch.equal(a, r)
+
+
+def test_backward_twice(dev):
+    """The saved rows go with the first backward unless the graph is kept."""
+    from spotv2net_amd import layer_norm
+    x, w, b, dy = make(dev, 9, 40, torch.float32, torch.float32)
+    xs = x.detach().requires_grad_()
+    y = layer_norm(xs, w, b)
+    a = torch.autograd.grad(y, xs, dy, retain_graph=True)[0]
+    assert torch.equal(a, torch.autograd.grad(y, xs, dy)[0])
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(y, xs, dy)
+    # an input overwritten after the forward is noticed
+    xs = x.detach().clone().requires_grad_()
+    z = xs * 1.0
+    y = layer_norm(z, w, b)
+    z.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y, xs, dy)
