@@ -48,6 +48,7 @@ constexpr int NS_PARTS = 1024;  // most partial sums of squares of one matrix
 constexpr int NS_PART_ELEMS = 4096;
 constexpr int NS_EXACT = 32;    // smaller sides up to which the products are f32
 constexpr int NS_HALF = 128;    // tiles of 128 that are worth a round of their own
+constexpr int NS_FUSED = 512;   // tiles of 32 up to which blocks make their own rows of Q
 constexpr int NS_TINY = 72;     // tiles of 64 below which tiles of 32 are faster
 
 struct NsMat {
@@ -646,6 +647,97 @@ __global__ __launch_bounds__(64 * W, FT == 4 ? 1 : 2) void k_ns_mm(NsArgs A, NsS
   }
 }
 
+// ---- 3b: Q and X's product in one launch, for small matrices (mp <= 128) ----
+// A 32 x 32 tile of X needs 32 rows of Q, 32 x m values from the m x m S: each block
+// makes them itself (in LDS, as fragments) rather than wait for a launch that stores
+// Q.  128 x 1,024: 4.7 + 4.3 -> 6.2 us a step.  Eight waves: first Q's m / 32 tiles times
+// slices of their depth, then 16 K values of X's product each.
+template <int EPI, int PR>
+__global__ __launch_bounds__(512, 2) void k_ns_qx(NsArgs A, NsScale sc, int cur) {
+  constexpr int PL = PR == 3 ? 2 : 1;
+  __shared__ __attribute__((aligned(16))) float sum[8][16][64];
+  __shared__ __attribute__((aligned(16))) _Float16 qf[8][2][512];
+  const NsTile tl = ns_tile_of<32, EPI>(A, ns_xcd(blockIdx.x, gridDim.x));
+  const NsMat& M = *tl.M;
+  const int64_t xs = (int64_t)tl.bt * 2 * M.mp * M.np, ss = (int64_t)tl.bt * 2 * M.mp * M.mp;
+  const _Float16 *S = M.s + ss, *R = M.xt[cur] + xs;
+  const int lane = threadIdx.x & 63, wave = wave_id();
+  const int kp = M.mp, nk = kp / 16;       // 4 or 8
+  const int tiles = kp / 32, slices = 8 / tiles;
+  const int tq = wave % tiles, sl = wave / tiles;
+  auto product = [&](const f16x8* p, const f16x8* q, f32x16 c) {
+    if (PR == 3 && M.exact) return ns_mfma_exact(p, q, c);
+    return ns_mfma<PR>(p, q, c);
+  };
+  // X's fragment of this wave's K values, in flight meanwhile
+  f16x8 xb[2];
+#pragma unroll
+  for (int p = 0; p < PL; ++p)
+    xb[p] = *(const f16x8*)(R + ns_blk(tl.tj, min(wave, nk - 1), kp) + p * 512 + lane * 8);
+  f32x16 acc;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+  for (int k = sl; k < nk; k += slices) {
+    f16x8 a[2], b[2];
+#pragma unroll
+    for (int p = 0; p < PL; ++p) {
+      a[p] = *(const f16x8*)(S + ns_blk(tq, k, kp) + p * 512 + lane * 8);
+      b[p] = *(const f16x8*)(S + ns_blk(tl.ti, k, kp) + p * 512 + lane * 8);
+    }
+    acc = product(a, b, acc);
+  }
+#pragma unroll
+  for (int e = 0; e < 16; ++e) sum[wave][e][lane] = acc[e];
+  __syncthreads();
+  if (sl < 2) {
+    // (S S) is symmetric: the tile's transpose, whose lane & 31 is Q's row, is what the
+    // accumulators hold as fragments; slice sl finishes 16 of the tile's 32 K values
+    const NsOut o = ns_out<NS_Q>(sc, M);
+    const _Float16* p = S + ns_blk(tl.ti, tq * 2 + sl, kp) + lane * 8;
+    float old[8], v[8];
+    ns_unpack(*(const f16x8*)p, *(const f16x8*)(p + 512), M.exact, old);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float d = 0.f;
+      for (int u = 0; u < slices; ++u) d += sum[tq + tiles * u][sl * 8 + e][lane];
+      v[e] = fmaf(o.old, old[e], o.up * d);
+    }
+    f16x8 hi, lo;
+    ns_pack(v, M.exact, hi, lo);
+    *(f16x8*)&qf[tq * 2 + sl][0][lane * 8] = hi;
+    *(f16x8*)&qf[tq * 2 + sl][1][lane * 8] = lo;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+  if (wave < nk) {
+    f16x8 a[2];
+    a[0] = *(const f16x8*)&qf[wave][0][lane * 8];
+    a[1] = *(const f16x8*)&qf[wave][1][lane * 8];
+    acc = product(a, xb, acc);
+  }
+#pragma unroll
+  for (int e = 0; e < 16; ++e) sum[wave][e][lane] = acc[e];
+  __syncthreads();
+  // two elements a wave; slot 0 of an element is read by its own adder alone
+  float part[2];
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    part[q] = 0.f;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) part[q] += sum[u][wave * 2 + q][lane];
+  }
+#pragma unroll
+  for (int q = 0; q < 2; ++q) sum[0][wave * 2 + q][lane] = part[q];
+  __syncthreads();
+  if (wave != 0) return;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) acc[e] = sum[0][e][lane];
+  ns_wave_sync();
+  ns_epilogue<EPI>(acc, ns_out<EPI>(sc, M), M, sc, R, tl.bt, tl.ti * 32, tl.tj * 32, cur, true,
+                   &sum[1][0][0]);
+}
+
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
@@ -805,14 +897,31 @@ static void ns_product(NsArgs& A, const NsScale& sc, int cur, int pad, hipStream
   if (small > 0) ns_launch<EPI, 1, 8, PR>(A, sc, cur, small, -1, stream);
 }
 
+// Whether Q and X's product go in one launch: every matrix small enough for k_ns_qx, and
+// few enough tiles that each making its rows of Q costs less than a launch
+static bool ns_fused(NsArgs& A) {
+  for (int i = 0; i < A.count; ++i)
+    if (A.mat[i].mp > 128) return false;
+  return ns_count<NS_X>(A, 32, [](const NsMat&) { return true; }) <= NS_FUSED;
+}
+
 template <int PR>
 static void ns_one_step(NsArgs& A, const NsScale& sc, int s, bool last, int pad,
                         hipStream_t stream) {
   const int cur = s & 1;
   ns_product<NS_S, PR>(A, sc, cur, pad, stream);
+  if (ns_fused(A)) {
+    const int64_t n = ns_count<NS_X>(A, 32, [](const NsMat&) { return true; });
+    if (!last)
+      hipLaunchKernelGGL((k_ns_qx<NS_X, PR>), dim3((unsigned)n), dim3(512), 0, stream, A, sc, cur);
+    else if constexpr (PR == 3)  // (the last step keeps both planes)
+      hipLaunchKernelGGL((k_ns_qx<NS_LAST, PR>), dim3((unsigned)n), dim3(512), 0, stream, A, sc,
+                         cur);
+    return;
+  }
   ns_product<NS_Q, PR>(A, sc, cur, pad, stream);
-  if (last) ns_product<NS_LAST, PR>(A, sc, cur, pad, stream);
-  else ns_product<NS_X, PR>(A, sc, cur, pad, stream);
+  if (!last) ns_product<NS_X, PR>(A, sc, cur, pad, stream);
+  else if constexpr (PR == 3) ns_product<NS_LAST, PR>(A, sc, cur, pad, stream);
 }
 
 // Steps at the start that may use the hi planes alone, where the result is bf16: with
