@@ -46,7 +46,9 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 constexpr int NS_MAX = 16;      // matrices of one launch
 constexpr int NS_PARTS = 1024;  // most partial sums of squares of one matrix
 constexpr int NS_PART_ELEMS = 4096;
+constexpr int NS_THIN_COLS = 128;  // columns of a thin matrix a block keeps
 constexpr int NS_EXACT = 32;    // smaller sides up to which the products are f32
+constexpr int NS_THIN_LONG = 2048;  // length from which a thin matrix has launches of its own
 constexpr int NS_HALF = 128;    // tiles of 128 that are worth a round of their own
 constexpr int NS_FUSED = 512;   // tiles of 32 up to which blocks make their own rows of Q
 constexpr int NS_TINY = 72;     // tiles of 64 below which tiles of 32 are faster
@@ -65,6 +67,7 @@ struct NsMat {
   float lr;             // the update's factor (with buf)
   _Float16 *x, *xt[2], *s, *q;
   double* part;         // [batch][parts]
+  float* thin;          // k_ns_thin's partial S [2][batch][np / NS_THIN_COLS][1024], or NULL
 };
 struct NsArgs {
   NsMat mat[NS_MAX];
@@ -738,6 +741,163 @@ __global__ __launch_bounds__(512, 2) void k_ns_qx(NsArgs A, NsScale sc, int cur)
                    &sum[1][0][0]);
 }
 
+// ---- 4: thin matrices (m <= 32), one launch a step ----
+// X is at most 32 rows tall, so a block keeps 128 of its n columns in registers, f32, and
+// needs of the others only S: a launch adds the blocks' partial S in block order, makes
+// Q, its columns of X' and its partial of the next S, all with f32 matrix instructions.
+// A wave has 32 columns as accumulators hold them (lane & 31 the column, register e and
+// lane half h the row 8·(e/4) + 4h + e%4), and S and Q the same way: S is symmetric, so
+// instruction e of S S and of Q X takes register e of both operands as it is.  Only X Xt
+// sums over columns and turns them in LDS.  A matrix of at most 128 columns takes all its
+// steps in one launch.
+// steps: how many this launch takes; first: from the caller's matrix (else from M.x);
+// last: the result goes to the caller.  single: one block per matrix.
+template <typename T>
+__global__ __launch_bounds__(256) void k_ns_thin(NsArgs A, NsScale sc, int cur, int steps,
+                                                 int first, int last, int single) {
+  constexpr int CC = NS_THIN_COLS;
+  __shared__ float xs[4][32][33];        // a wave's columns, turned
+  __shared__ float red[2][4][16][64];    // the waves' sums of X Xt, two steps in turn
+  __shared__ double nred[4];
+  const int mi = ns_find(A, blockIdx.x);
+  const NsMat& M = A.mat[mi];
+  const int local = blockIdx.x - A.first[mi];
+  const int chunks = M.np / CC;
+  const int bt = local / chunks, ch = local - bt * chunks;
+  const int t = threadIdx.x, lane = t & 63, h = lane >> 5, wave = wave_id();
+  const int j = ch * CC + wave * 32 + (lane & 31);
+  auto row_of = [&](int e) { return 8 * (e >> 2) + 4 * h + (e & 3); };
+  float* X = (float*)M.x + (int64_t)bt * 32 * M.np;
+  const float* part_in = M.thin + ((int64_t)cur * M.batch + bt) * chunks * 1024;
+  float* part_out = M.thin + ((int64_t)(cur ^ 1) * M.batch + bt) * chunks * 1024;
+  f32x16 x;
+  if (first) {
+    const T* g = (const T*)M.g + bt * M.g_batch;
+    float m[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int i = row_of(e);
+      const int64_t row = M.flip ? j : i, col = M.flip ? i : j;
+      const bool in = i < M.m && j < M.n;
+      x[e] = in ? (float)g[row * M.ld + col] : 0.f;
+      m[e] = in && M.buf ? M.buf[row * M.cols + col] : 0.f;
+    }
+    double acc = 0.0;
+    for (int k = t; k < M.parts; k += 256) acc += M.part[(int64_t)bt * M.parts + k];
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) acc += __shfl_xor(acc, o, 64);
+    if (lane == 0) nred[wave] = acc;
+    __syncthreads();
+    const double norm = sqrt((nred[0] + nred[1]) + (nred[2] + nred[3]));
+    const double inv = 1.0 / (norm < (double)sc.eps ? (double)sc.eps : norm);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float u = M.buf ? ns_update(sc, x[e], m[e]) : x[e];
+      x[e] = (float)((double)u * inv);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[e] = X[(int64_t)row_of(e) * M.np + j];
+  }
+  // the wave's columns of X Xt
+  auto gram = [&]() {
+    f32x16 acc;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      acc[e] = 0.f;
+      xs[wave][row_of(e)][lane & 31] = x[e];
+    }
+    ns_wave_sync();
+#pragma unroll
+    for (int q = 0; q < 16; ++q) {
+      const float a = xs[wave][lane & 31][2 * q + h];
+      acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a, a, acc, 0, 0, 0);
+    }
+    ns_wave_sync();
+    return acc;
+  };
+  // the block's: in every wave's registers (single), or to its partial
+  auto reduce = [&](const f32x16& acc, int buf, f32x16* S) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) red[buf][wave][e][lane] = acc[e];
+    __syncthreads();
+    if (single) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        (*S)[e] = (red[buf][0][e][lane] + red[buf][1][e][lane]) +
+                  (red[buf][2][e][lane] + red[buf][3][e][lane]);
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int e = wave * 4 + q;
+        part_out[(int64_t)ch * 1024 + e * 64 + lane] =
+            (red[buf][0][e][lane] + red[buf][1][e][lane]) +
+            (red[buf][2][e][lane] + red[buf][3][e][lane]);
+      }
+    }
+  };
+  f32x16 S;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) S[e] = 0.f;
+  int buf = 0;
+  if (first) {
+    reduce(gram(), buf, &S);
+    buf ^= 1;
+  } else {
+    // the blocks' partials: a wave adds four registers' worth and hands them round
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    const float* p = part_in + wave * 256 + lane;
+#pragma unroll 4
+    for (int k = 0; k < chunks; ++k)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[q] += p[(int64_t)k * 1024 + q * 64];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) red[buf][0][wave * 4 + q][lane] = v[q];
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 16; ++e) S[e] = red[buf][0][e][lane];
+    buf ^= 1;
+  }
+  for (int s = 0; s < steps; ++s) {
+    f32x16 Q, y;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) Q[e] = 0.f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) Q = __builtin_amdgcn_mfma_f32_32x32x2f32(S[e], S[e], Q, 0, 0, 0);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      Q[e] = fmaf(sc.c, Q[e], sc.b * S[e]);
+      y[e] = 0.f;
+    }
+    // (a x joins the finished sum: under it, every addition would round at its size)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) y = __builtin_amdgcn_mfma_f32_32x32x2f32(Q[e], x[e], y, 0, 0, 0);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[e] = fmaf(sc.a, x[e], y[e]);
+    if (last && s + 1 == steps) break;
+    reduce(gram(), buf, &S);
+    buf ^= 1;
+  }
+  if (!last) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) X[(int64_t)row_of(e) * M.np + j] = x[e];
+    return;
+  }
+  const int64_t base = (int64_t)bt * M.rows * M.cols;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const int i = row_of(e);
+    if (i >= M.m || j >= M.n) continue;
+    const int64_t at = base + (M.flip ? (int64_t)j * M.cols + i : (int64_t)i * M.cols + j);
+    if (M.buf) {
+      float* w = (float*)M.out + at;
+      *w = fmaf(sc.keep, *w, -M.lr * x[e]);
+    } else {
+      ((T*)M.out)[at] = (T)x[e];
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
@@ -814,10 +974,29 @@ static int ns_pad(const NsMat* mats, int count) {
   return tiles >= NS_HALF ? 128 : 64;
 }
 
+// Whether a group's matrices of m <= NS_EXACT go to k_ns_thin: always where the others
+// (if any) take tiles above 32 or one is longer than NS_THIN_LONG; beside small matrices
+// they ride in those launches as exact tiles instead of adding their own.
+static bool ns_thin(const NsMat* mats, int count) {
+  int64_t tiles = 0;
+  bool others = false, any = false, longer = false;
+  for (int i = 0; i < count; ++i) {
+    if (mats[i].exact) {
+      any = true;
+      longer |= mats[i].n > NS_THIN_LONG;
+    } else {
+      others = true;
+      tiles += (int64_t)mats[i].batch * (ns_up(mats[i].m, 64) / 64) * (ns_up(mats[i].n, 64) / 64);
+    }
+  }
+  return any && (!others || longer || tiles >= NS_TINY);
+}
+
 // pads the shapes and lays its workspace out from `ws`
 // (NULL: only counts); returns the bytes
 static int64_t ns_plan(NsMat* mats, int count, int pad, char* ws) {
   int64_t off = 0;
+  const bool thin = ns_thin(mats, count);
   auto take = [&](int64_t bytes) {
     char* p = ws ? ws + off : nullptr;
     off += ns_up(bytes, 256);
@@ -825,6 +1004,15 @@ static int64_t ns_plan(NsMat* mats, int count, int pad, char* ws) {
   };
   for (int i = 0; i < count; ++i) {
     NsMat& M = mats[i];
+    M.thin = nullptr;
+    if (thin && M.exact) {
+      M.mp = NS_EXACT;
+      M.np = (int)ns_up(M.n, NS_THIN_COLS);
+      M.part = (double*)take((int64_t)M.batch * M.parts * 8);
+      M.x = (_Float16*)take((int64_t)M.batch * NS_EXACT * M.np * 4);
+      M.thin = (float*)take((int64_t)2 * M.batch * (M.np / NS_THIN_COLS) * 4096);
+      continue;
+    }
     M.mp = (int)ns_up(M.m, pad);
     M.np = (int)ns_up(M.n, pad);
     const int64_t xb = (int64_t)M.batch * M.mp * M.np * 4, sb = (int64_t)M.batch * M.mp * M.mp * 4;
@@ -936,21 +1124,45 @@ static int ns_cheap(const NsMat& M, const NsScale& sc, int steps) {
   return std::max(0, std::min(h, steps - 2));
 }
 
-static int ns_run(NsArgs& A, const NsScale& sc, int steps, int pad, hipStream_t stream) {
+template <typename T>
+static void ns_run_as(NsArgs& A, const NsScale& sc, int steps, int pad, hipStream_t stream) {
   int64_t n = ns_blocks(A, [](const NsMat& M) -> int64_t { return M.parts; });
-  const int dtype = A.mat[0].dtype;  // one for the whole group
-  auto* norm = dtype == SV2N_DT_F32 ? k_ns_norm<float>
-             : dtype == SV2N_DT_BF16 ? k_ns_norm<__bf16> : k_ns_norm<_Float16>;
-  auto* split = dtype == SV2N_DT_F32 ? k_ns_split<float>
-              : dtype == SV2N_DT_BF16 ? k_ns_split<__bf16> : k_ns_split<_Float16>;
-  hipLaunchKernelGGL(norm, dim3((unsigned)n), dim3(256), 0, stream, A, sc);
-  n = ns_blocks(A, [](const NsMat& M) -> int64_t { return (int64_t)(M.mp / 64) * (M.np / 64); });
-  hipLaunchKernelGGL(split, dim3((unsigned)n), dim3(256), 0, stream, A, sc);
-  const int cheap = ns_cheap(A.mat[0], sc, steps);  // (16-bit types come one matrix a call)
-  for (int k = 0; k < steps; ++k) {
-    if (k < cheap) ns_one_step<1>(A, sc, k, false, pad, stream);
-    else ns_one_step<3>(A, sc, k, k + 1 == steps, pad, stream);
+  hipLaunchKernelGGL(k_ns_norm<T>, dim3((unsigned)n), dim3(256), 0, stream, A, sc);
+  NsArgs B{}, H{};  // tiles, thin
+  for (int i = 0; i < A.count; ++i) {
+    NsArgs& to = A.mat[i].thin ? H : B;
+    to.mat[to.count++] = A.mat[i];
   }
+  if (H.count) {
+    n = ns_blocks(H, [](const NsMat& M) -> int64_t { return M.np / NS_THIN_COLS; });
+    bool single = true;
+    for (int i = 0; i < H.count; ++i) single &= H.mat[i].np == NS_THIN_COLS;
+    auto go = [&](int cur, int k, int first, int last) {
+      hipLaunchKernelGGL(k_ns_thin<T>, dim3((unsigned)n), dim3(256), 0, stream, H, sc, cur, k, first,
+                         last, (int)single);
+    };
+    if (single) {
+      go(0, steps, 1, 1);
+    } else {
+      go(1, 0, 1, 0);
+      for (int k = 0; k < steps; ++k) go(k & 1, 1, 0, k + 1 == steps);
+    }
+  }
+  if (!B.count) return;
+  n = ns_blocks(B, [](const NsMat& M) -> int64_t { return (int64_t)(M.mp / 64) * (M.np / 64); });
+  hipLaunchKernelGGL(k_ns_split<T>, dim3((unsigned)n), dim3(256), 0, stream, B, sc);
+  const int cheap = ns_cheap(B.mat[0], sc, steps);  // (16-bit types come one matrix a call)
+  for (int k = 0; k < steps; ++k) {
+    if (k < cheap) ns_one_step<1>(B, sc, k, false, pad, stream);
+    else ns_one_step<3>(B, sc, k, k + 1 == steps, pad, stream);
+  }
+}
+
+static int ns_run(NsArgs& A, const NsScale& sc, int steps, int pad, hipStream_t stream) {
+  const int dtype = A.mat[0].dtype;  // one for the whole group
+  if (dtype == SV2N_DT_F32) ns_run_as<float>(A, sc, steps, pad, stream);
+  else if (dtype == SV2N_DT_BF16) ns_run_as<__bf16>(A, sc, steps, pad, stream);
+  else ns_run_as<_Float16>(A, sc, steps, pad, stream);
   return (int)hipGetLastError();
 }
 

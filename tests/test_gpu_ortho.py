@@ -63,7 +63,8 @@ def check(g, **kw):
 
 SHAPES = [(1, 1), (1, 7), (7, 1), (2, 2), (3, 130), (30, 30), (31, 33), (64, 64), (65, 64),
           (128, 12), (128, 128), (129, 127), (200, 126), (400, 1260), (1024, 128), (777, 1537),
-          (1300, 1300), (1, 4096), (4096, 5)]
+          (1300, 1300), (1, 4096), (4096, 5), (32, 128), (32, 129), (128, 32), (17, 127), (31, 2049),
+          (16384, 3), (32, 5000), (33, 5000)]
 
 
 @pytest.mark.parametrize("rows,cols", SHAPES)
@@ -135,7 +136,7 @@ def test_step_counts(dev, steps):
     check(gradient(dev, 700, 900), steps=steps)
 
 
-@pytest.mark.parametrize("batch,rows,cols", [(1, 40, 50), (5, 33, 70), (3, 300, 140), (17, 16, 16),
+@pytest.mark.parametrize("batch,rows,cols", [(1, 40, 50), (5, 33, 70), (3, 300, 140), (17, 16, 16), (9, 3, 700), (4, 1500, 30),
                                              (2, 800, 1100)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_stacks_are_their_matrices(dev, batch, rows, cols, dtype):

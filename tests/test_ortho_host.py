@@ -63,11 +63,16 @@ def test_workspace():
     lib = _lib().load()
     assert lib.sv2n_orthogonalize_workspace(1, 0, 8) == 0
     assert lib.sv2n_orthogonalize_workspace(1, 8, 16385) == 0
-    for b, m, n in ((1, 1, 1), (3, 1537, 777), (1, 128, 1024), (6, 2048, 2048)):
+    for b, m, n in ((1, 1, 1), (2, 4096, 20)):
+        # thin matrices: 32 rows of f32 and two partial S per 128 columns
+        w = -(-max(m, n) // 128)
+        assert b * w * (32 * 128 + 2 * 1024) * 4 <= lib.sv2n_orthogonalize_workspace(b, m, n) <= \
+            b * w * (32 * 128 + 2 * 1024) * 4 + b * 1024 * 8 + 4 * 256
+    for b, m, n in ((1, 33, 33), (3, 1537, 777), (1, 128, 1024), (6, 2048, 2048)):
         lo, hi = min(m, n), max(m, n)
         # X, its two transposes, S and Q at 4 B, padded to at most 128 a side
         least = b * 4 * (3 * lo * hi + 2 * lo * lo)
-        most = b * 4 * (3 * (lo + 127) * (hi + 127) + 2 * (lo + 127) ** 2) + b * 512 * 8 + 6 * 256
+        most = b * 4 * (3 * (lo + 127) * (hi + 127) + 2 * (lo + 127) ** 2) + b * 1024 * 8 + 6 * 256
         assert least <= lib.sv2n_orthogonalize_workspace(b, m, n) <= most
         assert lib.sv2n_orthogonalize_workspace(b, m, n) == lib.sv2n_orthogonalize_workspace(b, n, m) \
             or m != n
