@@ -24,9 +24,10 @@
 // The next row's loads are in flight while a row is summed, clamped to the last row
 // instead of branching; a group past the last row adds zeros.
 //
-// MI355X, us (forward / backward with its second launch; a copy reaches 5.0 TB/s):
-//   15,360 x 400 f32      13.3 / 20.0        16,384 x 4,096 f32   97 / 161
-//   262,144 x 128 f32       52 / 79          16,384 x 8,192 bf16 106 / 268
+// MI355X, us (forward / backward with its second launch; a large copy reaches 5.0 TB/s):
+//   15,360 x 400 f32      11.3 / 18.7        16,384 x 4,096 f32    91 / 163  (5.9 / 5.1 TB/s)
+//   262,144 x 128 f32       45 / 82          16,384 x 8,192 bf16   97 / 160  (5.6 / 5.2 TB/s)
+//   3,840 x 3,000 bf16    12.6 / 28.3        10,007 x 1,261 f16  17.4 / 26.7
 #include "sv2n_common.h"
 #include <algorithm>
 #include <type_traits>

@@ -34,6 +34,7 @@
 //
 // Several matrices (a model's weights) share each launch: `first` maps blocks to
 // matrices, so a step over four weights costs the same 3·steps + 2 launches as one.
+// Small and thin matrices take fewer (k_ns_qx, k_ns_thin).
 #include "sv2n_common.h"
 #include <algorithm>
 #include <cmath>
@@ -477,8 +478,9 @@ __device__ __forceinline__ f32x16 ns_mfma(const f16x8* a, const f16x8* b, f32x16
 // from big0 on, what whole rounds of FT = 4 left.
 template <int EPI, int FT, int W, int PR>
 __global__ __launch_bounds__(64 * W, FT == 4 ? 1 : 2) void k_ns_mm(NsArgs A, NsScale sc, int cur, int big0) {
-  // (deeper does not help: 2 to 5 steps measure the same, what bounds FT = 1 and 2 is how
-  // many lines a CU can have on the way from the L2)
+  // (deeper does not help: 2 to 5 steps measure the same.  FT = 1 and 2 are bound by the
+  // 64 B a cycle that a CU's L1 hands its registers: with every load a hit they take 80 %
+  // of the time, and without the products 90 to 100 %)
   constexpr int DEPTH = FT == 4 ? (PR == 3 ? 2 : 4) : FT == 2 ? 2 : 4;
   constexpr int PL = PR == 3 ? 2 : 1;
   constexpr int TB = 32 * FT;
@@ -653,7 +655,8 @@ __global__ __launch_bounds__(64 * W, FT == 4 ? 1 : 2) void k_ns_mm(NsArgs A, NsS
 // ---- 3b: Q and X's product in one launch, for small matrices (mp <= 128) ----
 // A 32 x 32 tile of X needs 32 rows of Q, 32 x m values from the m x m S: each block
 // makes them itself (in LDS, as fragments) rather than wait for a launch that stores
-// Q.  128 x 1,024: 4.7 + 4.3 -> 6.2 us a step.  Eight waves: first Q's m / 32 tiles times
+// Q.  128 x 1,024: 4.3 + 4.5 us in two launches, 7.9 in one (92 -> 81 us with all steps).
+// Eight waves: first Q's m / 32 tiles times
 // slices of their depth, then 16 K values of X's product each.
 template <int EPI, int PR>
 __global__ __launch_bounds__(512, 2) void k_ns_qx(NsArgs A, NsScale sc, int cur) {
@@ -749,7 +752,8 @@ __global__ __launch_bounds__(512, 2) void k_ns_qx(NsArgs A, NsScale sc, int cur)
 // lane half h the row 8·(e/4) + 4h + e%4), and S and Q the same way: S is symmetric, so
 // instruction e of S S and of Q X takes register e of both operands as it is.  Only X Xt
 // sums over columns and turns them in LDS.  A matrix of at most 128 columns takes all its
-// steps in one launch.
+// steps in one launch.  Against three products a step on tiles, us: 16 x 128 66 -> 21,
+// 32 x 1,024 87 -> 43, 16 x 4,096 187 -> 53 (what is left is launches).
 // steps: how many this launch takes; first: from the caller's matrix (else from M.x);
 // last: the result goes to the caller.  single: one block per matrix.
 template <typename T>

@@ -21,6 +21,7 @@ CovarianceLaggedDataset windows, utils/dataset.py:200-282).
 from __future__ import annotations
 
 import ctypes
+import math
 from typing import List, Optional
 
 import torch
@@ -1341,7 +1342,7 @@ NS_MAX_SIDE, NS_MAX_BATCH, NS_MAX_STEPS = 16384, 1024, 32  # SV2N_NS_MAX_*
 
 def _ns_check(steps, eps) -> None:
     _need(1 <= steps <= NS_MAX_STEPS, f"orthogonalize: 1 to {NS_MAX_STEPS} steps, got {steps}")
-    _need(eps > 0.0, f"orthogonalize: eps must be positive, got {eps}")
+    _need(0.0 < eps < math.inf, f"orthogonalize: eps must be positive, got {eps}")
 
 
 def _ns_rc(rc: int, what: str) -> None:
@@ -1405,6 +1406,9 @@ def _muon_step(weights, grads, momenta, lr_scales, lr, momentum, nesterov, weigh
     _need(len(grads) == len(momenta) == len(lr_scales) == k, "muon_step: lists of different lengths")
     _ns_check(steps, eps)
     _need(0.0 <= momentum < 1.0, f"muon_step: momentum must be in [0, 1), got {momentum}")
+    _need(math.isfinite(lr) and math.isfinite(weight_decay) and
+          all(math.isfinite(s) for s in lr_scales),
+          f"muon_step: lr {lr} and weight_decay {weight_decay} must be finite")
     mats, scales = [], []
     for w, g, m, s in zip(weights, grads, momenta, lr_scales):
         _f32(w, g, m)

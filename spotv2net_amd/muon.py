@@ -71,13 +71,16 @@ def muon_step(weights: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
     torch.ops.sv2n.muon_step(weights, grads, momenta,
                              [lr_scale(w.shape[0], w.shape[1], adjust_lr) for w in weights], lr,
                              momentum, nesterov, weight_decay, steps, a, b, c, eps)
+    # the kernels write through raw pointers: autograd learns of it here
+    torch.autograd.graph.increment_version(weights + momenta)
 
 
 class Muon(torch.optim.Optimizer):
     """Momentum with orthogonalised updates for weight matrices (2-D float32
     parameters); everything else belongs to another optimiser.  One ``step`` is
-    ``3 steps + 2`` launches per 16 matrices of a parameter group, without a host
-    synchronisation, and can be captured into a graph."""
+    at most ``3 steps + 2`` launches per 16 matrices of a parameter group (a few more
+    where thin ones stand beside large ones), without a host synchronisation, and can
+    be captured into a graph after a first step outside of it."""
 
     def __init__(self, params, lr: float = 1e-3, weight_decay: float = 0.1, momentum: float = 0.95,
                  nesterov: bool = True, coefficients: Tuple[float, float, float] = COEFFICIENTS,
@@ -104,6 +107,10 @@ class Muon(torch.optim.Optimizer):
             ws = [p for p in group["params"] if p.grad is not None]
             for p in ws:
                 if "momentum_buffer" not in self.state[p]:
+                    if p.is_cuda and torch.cuda.is_current_stream_capturing():
+                        # its zeros would be part of the graph, and of every replay
+                        raise RuntimeError("Muon: run one step before capturing one (the "
+                                           "momentum is allocated by the first)")
                     self.state[p]["momentum_buffer"] = torch.zeros_like(
                         p, memory_format=torch.contiguous_format)
             muon_step(ws, [p.grad for p in ws], [self.state[p]["momentum_buffer"] for p in ws],

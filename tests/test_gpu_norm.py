@@ -354,3 +354,19 @@ def test_backward_twice(dev):
     z.add_(1.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         torch.autograd.grad(y, xs, dy)
+
+
+def test_past_32_bit_offsets(dev):
+    """More than 2^31 elements: the last rows as if they stood alone."""
+    from spotv2net_amd import layer_norm
+    rows, cols = 262151, 8200
+    x = torch.empty(rows, cols, device=dev, dtype=torch.bfloat16).normal_()
+    w = torch.randn(cols, device=dev)
+    b = torch.randn(cols, device=dev)
+    xs = x.requires_grad_()
+    y = layer_norm(xs, w, b)
+    (dx,) = torch.autograd.grad(y, xs, x.detach())
+    tail = x.detach()[-7:].clone().requires_grad_()
+    yt = layer_norm(tail, w, b)
+    (dxt,) = torch.autograd.grad(yt, tail, tail.detach())
+    assert torch.equal(y[-7:], yt) and torch.equal(dx[-7:], dxt)

@@ -60,7 +60,7 @@ def named(model, ref):
 
 @pytest.mark.parametrize("hidden,heads,act,n", [
     ((16, 8), 4, "tanh", 30), ((12,), 3, "sigmoid", 30), ((8, 8, 5), 2, "tanh", 17),
-    ((16, 16, 16), 8, "tanh", 40), ((33, 7), 1, "sigmoid", 30)])
+    ((16, 16, 16), 8, "tanh", 40), ((8, 8, 5), 2, "sigmoid", 40), ((33, 7), 1, "sigmoid", 30)])
 def test_model_matches_oracle(dev, hidden, heads, act, n):
     """Forward and every gradient, on the n <= 32 and the larger-graph attention."""
     from spotv2net_amd import synthetic_batch
@@ -258,3 +258,69 @@ def test_fit_with_muon(dev):
         rec = f.run_epoch()
         assert math.isfinite(rec["train_loss"]) and math.isfinite(rec["test_loss"])
     assert not torch.equal(model.gat_layers[0].lin_src.weight, w0)
+
+
+def test_fit_bf16(dev):
+    """The bf16 mode's own layer-0 operands (x gathered as its bf16 twin alone) with a
+    norm behind them."""
+    from spotv2net_amd import GATModel, WindowDataset, synthetic_series
+    from spotv2net_amd.train import Fit
+    torch.manual_seed(0)
+    vol, volvol = synthetic_series(110, n=30, seed=1)
+    ds = WindowDataset(vol.to(dev), volvol.to(dev), 4)
+    model = GATModel(120, 12, 6, 1, [64], concat_heads=True, layer_norm=True).to(dev)
+    model.set_precision("bf16")
+    f = Fit(model, ds, 64, lr=1e-3, optimizer="muon")
+    a, b = f.run_epoch(), f.run_epoch()
+    assert all(math.isfinite(r[k]) for r in (a, b) for k in ("train_loss", "test_loss"))
+
+
+def test_compiled_model(dev):
+    from spotv2net_amd import synthetic_batch
+    model, _ = build(dev, hidden=(16, 8))
+    data = synthetic_batch(2, 2, seed=1, device=dev)
+    want = model(data)
+    got = torch.compile(model, backend="aot_eager")(data)
+    assert_close(got, want, what="compiled")
+
+
+def _rank(rank, world, port, out_dir):
+    import os
+    import torch.distributed as dist
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    torch.cuda.set_device(0)
+    dev = torch.device("cuda", 0)
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    try:
+        from spotv2net_amd import synthetic_batch
+        from spotv2net_amd.train import TrainStep, broadcast_params_
+        model = build(dev, hidden=(16, 8), seed=20 + rank)[0].train()
+        broadcast_params_(model, 0)
+        data = synthetic_batch(4, 2, seed=70 + rank, device=dev)
+        step = TrainStep(model, data, lr=1e-2, use_graph=True, optimizer="muon")
+        assert step.distributed and step._shapes[0].g_opt is not None
+        for _ in range(3):
+            step()
+        torch.cuda.synchronize()
+        torch.save({k: v.detach().cpu() for k, v in model.state_dict().items()},
+                   os.path.join(out_dir, f"rank{rank}.pt"))
+    finally:
+        dist.destroy_process_group()
+
+
+def test_two_ranks_stay_identical(dev, tmp_path):
+    """Two data-parallel ranks (gloo, sharing the GPU) under Muon: the replicas end bit
+    for bit the same, and moved."""
+    import socket
+
+    import torch.multiprocessing as mp
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    mp.start_processes(_rank, args=(2, port, str(tmp_path)), nprocs=2, join=True,
+                       start_method="spawn")
+    r0, r1 = (torch.load(tmp_path / f"rank{r}.pt", weights_only=True) for r in range(2))
+    start = build(torch.device("cpu"), hidden=(16, 8), seed=20)[0].state_dict()
+    for k in r0:
+        assert torch.equal(r0[k], r1[k]), k
+    assert not torch.equal(r0["gat_layers.0.lin_src.weight"], start["gat_layers.0.lin_src.weight"])

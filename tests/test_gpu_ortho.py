@@ -221,6 +221,9 @@ def test_refusals(dev):
                       (([w], [g], [b.cpu()]), "device")):
         with pytest.raises(RuntimeError, match=msg):
             muon_step(*args, lr=0.1)
+    for kw in (dict(lr=float("nan")), dict(lr=0.1, weight_decay=float("inf"))):
+        with pytest.raises(RuntimeError, match="must be finite"):
+            muon_step([w], [g], [b], **kw)
     with pytest.raises(RuntimeError, match="momentum must be"):
         muon_step([w], [g], [b], lr=0.1, momentum=1.0)
     with pytest.raises(ValueError, match="matrices"):
@@ -392,3 +395,67 @@ def test_opcheck(dev):
     ws, gs, ms = matrices(dev, [(20, 30), (8, 8)])
     torch.library.opcheck(ops.muon_step, (ws, gs, ms, [1.0, 1.0], 0.02, 0.95, True, 0.1, 5, *NS,
                                           1e-7), test_utils=utils)
+
+
+def test_past_32_bit_offsets(dev):
+    """Matrices of a stack, and rows of a matrix, more than 2^31 elements apart."""
+    from spotv2net_amd import orthogonalize
+    far = (1 << 31) + 77
+    buf = torch.empty(2 * far + 70 * 90, device=dev, dtype=torch.bfloat16)
+    st = torch.as_strided(buf, (3, 70, 90), (far, 90, 1))
+    g = gradient(dev, 3 * 70, 90, torch.bfloat16).view(3, 70, 90)
+    st.copy_(g)
+    assert torch.equal(orthogonalize(st), orthogonalize(g))
+    rows = torch.as_strided(buf, (3, 90), (far, 1))
+    assert torch.equal(orthogonalize(rows), orthogonalize(rows.contiguous()))
+    rows = torch.as_strided(buf, (3, 2), (far, 1))
+    assert torch.equal(orthogonalize(rows), orthogonalize(rows.contiguous()))
+
+
+def test_autograd_notices_the_update(dev):
+    """A weight saved for a backward and then stepped: the backward refuses."""
+    from spotv2net_amd import muon_step
+    w = gradient(dev, 8, 8).requires_grad_()
+    y = (w * w).sum()
+    muon_step([w], [gradient(dev, 8, 8, seed=1)], [torch.zeros(8, 8, device=dev)], lr=0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_first_step_is_not_captured(dev, monkeypatch):
+    from spotv2net_amd import Muon
+    p = torch.nn.Parameter(gradient(dev, 8, 8))
+    p.grad = gradient(dev, 8, 8, seed=1)
+    opt = Muon([p], lr=0.1)
+    with monkeypatch.context() as m:
+        m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        with pytest.raises(RuntimeError, match="one step before"):
+            opt.step()
+    opt.step()
+    with monkeypatch.context() as m:
+        m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        opt.step()
+
+
+def test_captured_large_products(dev):
+    """The kernels of large and of thin matrices in one captured step, replayed."""
+    from spotv2net_amd import muon_step
+    shapes = [(1500, 1600), (9, 3000), (40, 300), (6, 6)]
+    ws, gs, ms = matrices(dev, shapes)
+    ew, em = [w.clone() for w in ws], [m.clone() for m in ms]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        muon_step([w.clone() for w in ws], gs, [m.clone() for m in ms], lr=0.02)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        muon_step(ws, gs, ms, lr=0.02)
+    for k in range(3):
+        for i, g in enumerate(gs):
+            g.copy_(gradient(dev, *shapes[i], seed=300 + 7 * k + i))
+        graph.replay()
+        muon_step(ew, gs, em, lr=0.02)
+        torch.cuda.synchronize()
+        for a, b in zip(ws + ms, ew + em):
+            assert torch.equal(a, b), k
