@@ -514,7 +514,7 @@ __global__ __launch_bounds__(64 * W, FT == 4 ? 1 : 2) void k_ns_mm(NsArgs A, NsS
     for (int y = 0; y < FT; ++y)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[x][y][e] = 0.f;
-  const int nk = kp / 16;
+  const int nk = ((EPI == NS_S ? M.n : M.m) + 15) / 16;  // (the padding's zeros add nothing)
   auto fetch = [&](int d, int k) {
 #pragma unroll
     for (int x = 0; x < FT; ++x)
