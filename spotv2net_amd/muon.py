@@ -72,7 +72,9 @@ def muon_step(weights: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
                              [lr_scale(w.shape[0], w.shape[1], adjust_lr) for w in weights], lr,
                              momentum, nesterov, weight_decay, steps, a, b, c, eps)
     # the kernels write through raw pointers: autograd learns of it here
-    torch.autograd.graph.increment_version(weights + momenta)
+    # (inference tensors have no version to raise)
+    torch.autograd.graph.increment_version(
+        [t for t in weights + momenta if not t.is_inference()])
 
 
 class Muon(torch.optim.Optimizer):

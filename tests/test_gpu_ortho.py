@@ -422,6 +422,18 @@ def test_autograd_notices_the_update(dev):
         y.backward()
 
 
+def test_inference_tensors(dev):
+    """Tensors of inference mode have no version: stepped like others."""
+    from spotv2net_amd import muon_step
+    w, g = gradient(dev, 8, 8), gradient(dev, 8, 8, seed=1)
+    want, m = w.clone(), torch.zeros(8, 8, device=dev)
+    muon_step([want], [g], [m], lr=0.1)
+    with torch.inference_mode():
+        got, m = w.clone(), torch.zeros(8, 8, device=dev)
+        muon_step([got], [g], [m], lr=0.1)
+    assert torch.equal(got, want)
+
+
 def test_first_step_is_not_captured(dev, monkeypatch):
     from spotv2net_amd import Muon
     p = torch.nn.Parameter(gradient(dev, 8, 8))
