@@ -8,8 +8,10 @@
 // their addresses to sv2n_torch_bind before the first call.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
@@ -139,6 +141,11 @@ Tensor backward_into(const Tensor& dy, const Tensor& x, const OptTensor& weight,
     TORCH_CHECK(dtype_code(v.scalar_type()) == wdt,
                 "sv2n: layer_norm_bwd: gradients and weight of different types");
   }
+  if (dw && db) {
+    const auto a = (uintptr_t)dw->const_data_ptr(), b = (uintptr_t)db->const_data_ptr();
+    const uintptr_t n = cols * dw->element_size();
+    TORCH_CHECK(a + n <= b || b + n <= a, "sv2n: layer_norm_bwd: the gradient buffers overlap");
+  }
   Tensor dx;
   if (need_dx) dx = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
   const bool wg = dw.has_value() || db.has_value();
@@ -211,10 +218,28 @@ struct LayerNormBackward : torch::autograd::Node {
 
   std::string name() const override { return "LayerNormBackward"; }
 
+  // A leaf's accumulation node lives as long as any graph of the leaf and keeps the
+  // stream it was made on.  If that is the default stream, the engine would make it wait
+  // for a stream that is being captured, which ends the process; here it is an error.
+  void refuse_capture_from_eager() {
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    for (uint32_t i = 0; i < num_outputs(); ++i) {
+      const auto& next = next_edge(i).function;
+      if (!task_should_compute_output(i) ||
+          !dynamic_cast<torch::autograd::AccumulateGrad*>(next.get()))
+        continue;
+      const auto s = next->stream();
+      TORCH_CHECK(!s || s->id() != c10::hip::getDefaultHIPStream(s->device_index()).id(),
+                  "sv2n: layer_norm's backward is being captured while an eager graph of the "
+                  "same leaf, built on the default stream, is alive: delete it first");
+    }
+  }
+
   variable_list apply(variable_list&& grads) override {
     variable_list out(3);
     if (!grads[0].defined()) return out;
     TORCH_CHECK(!released, torch::autograd::ERR_BACKWARD_TWICE);
+    refuse_capture_from_eager();
     const bool twice = at::GradMode::is_enabled();
     {
       at::AutoDispatchBelowAutograd below;
@@ -250,6 +275,9 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_autograd(const Tensor& x, const Op
   const bool need = at::GradMode::is_enabled() &&
                     (x.requires_grad() || (weight && weight->requires_grad()) ||
                      (bias && bias->requires_grad()));
+  for (const OptTensor& t : {OptTensor(x), weight, bias})
+    TORCH_CHECK(!torch::autograd::isFwGradDefined(t),
+                "sv2n: layer_norm has no forward-mode derivative");
   std::tuple<Tensor, Tensor, Tensor> out;
   {
     at::AutoDispatchBelowADInplaceOrView below;

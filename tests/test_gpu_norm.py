@@ -268,6 +268,38 @@ def test_replayed_graph(dev):
             assert torch.equal(a, r), k
 
 
+def test_capture_beside_an_eager_graph(dev):
+    """A backward captured while an eager graph of the same leaf is alive raises; once
+    that graph is gone the same capture runs."""
+    from spotv2net_amd import layer_norm
+    x, w, b, dy = make(dev, 64, 40, torch.float32, torch.float32)
+    xs = x.clone().requires_grad_()
+    keep = layer_norm(xs, w, b)
+
+    def step():
+        return torch.autograd.grad(layer_norm(xs, w, b), xs, dy)[0]
+
+    with pytest.raises(RuntimeError, match="eager graph"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            step()
+    want = torch.autograd.grad(keep, xs, dy)[0]
+    del keep
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    g.replay()
+    assert torch.equal(out, want)
+
+
+def test_gradient_buffers_must_not_overlap(dev):
+    x, w, b, dy = make(dev, 5, 40, torch.float32, torch.float32)
+    _, mean, rstd = torch.ops.sv2n.layer_norm(x, w, b, 1e-5)
+    buf = torch.zeros(60, device=dev)
+    for dw, db in ((buf[:40], buf[:40]), (buf[:40], buf[20:])):
+        with pytest.raises(RuntimeError, match="overlap"):
+            torch.ops.sv2n.layer_norm_bwd_acc(dy, x, w, mean, rstd, dw, db)
+
+
 def test_other_stream(dev):
     x, w, b, dy = make(dev, 2000, 777, torch.float32, torch.float32)
     want = run(x, w, b, dy)

@@ -73,6 +73,16 @@ def test_refuses_cpu_tensors():
         layer_norm(torch.randn(3, 4))
 
 
+def test_refuses_forward_mode():
+    import torch.autograd.forward_ad as fw
+    import spotv2net_amd  # noqa: F401
+    x, w = torch.randn(3, 4), torch.randn(4)
+    with fw.dual_level():
+        for args in ((fw.make_dual(x, x), w), (x, fw.make_dual(w, w))):
+            with pytest.raises(RuntimeError, match="no forward-mode"):
+                torch.ops.sv2n.layer_norm(*args, None, 1e-5)
+
+
 def test_fake_tensors_propagate_shapes():
     from torch._subclasses.fake_tensor import FakeTensorMode
     import spotv2net_amd  # noqa: F401
