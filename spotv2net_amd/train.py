@@ -28,6 +28,8 @@ from typing import Callable, Optional
 import torch
 import torch.distributed as dist
 
+from .graphed import _no_gc
+
 
 def _offsets(params, align: int):
     """Where each parameter starts in a flat buffer (a multiple of ``align``
@@ -415,18 +417,18 @@ class TrainStep:
         torch.cuda.synchronize()
         if self.distributed:
             sh.g_fb = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(sh.g_fb):
+            with _no_gc(), torch.cuda.graph(sh.g_fb):
                 self._fwd_bwd(sh)
             # the ÷ world size of the all-reduced sum rides in the optimizer
             # graph (no eager launch between the collective and the replay)
             ws = dist.get_world_size(self.group)
             sh.g_opt = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(sh.g_opt):
+            with _no_gc(), torch.cuda.graph(sh.g_opt):
                 self.flat.div_(ws)
                 self._opt_step()
         else:
             sh.g_fb = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(sh.g_fb):
+            with _no_gc(), torch.cuda.graph(sh.g_fb):
                 self._fwd_bwd(sh)
                 self._opt_step()
         torch.cuda.synchronize()
@@ -472,7 +474,7 @@ class ForwardStep:
             torch.cuda.synchronize()
             if use_graph:
                 self.graph = torch.cuda.CUDAGraph()
-                with torch.cuda.graph(self.graph):
+                with _no_gc(), torch.cuda.graph(self.graph):
                     self._run()
                 torch.cuda.synchronize()
             if self.out_sum is not None:

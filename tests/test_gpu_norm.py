@@ -9,6 +9,8 @@ step of its type."""
 import pytest
 import torch
 
+from spotv2net_amd.graphed import _no_gc
+
 pytestmark = pytest.mark.gpu
 
 U = 2.0 ** -24
@@ -254,7 +256,7 @@ def test_replayed_graph(dev):
         step()
     torch.cuda.current_stream().wait_stream(s)
     g = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(g):
+    with _no_gc(), torch.cuda.graph(g):
         out = step()
     for k in range(4):
         x2, _, _, dy2 = make(dev, 300, 400, torch.float32, torch.float32, seed=50 + k)
@@ -280,12 +282,12 @@ def test_capture_beside_an_eager_graph(dev):
         return torch.autograd.grad(layer_norm(xs, w, b), xs, dy)[0]
 
     with pytest.raises(RuntimeError, match="eager graph"):
-        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        with _no_gc(), torch.cuda.graph(torch.cuda.CUDAGraph()):
             step()
     want = torch.autograd.grad(keep, xs, dy)[0]
     del keep
     g = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(g):
+    with _no_gc(), torch.cuda.graph(g):
         out = step()
     g.replay()
     assert torch.equal(out, want)

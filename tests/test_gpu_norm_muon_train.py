@@ -225,6 +225,27 @@ def test_replays_equal_eager_steps(dev):
     assert keep.grad_fn is not None
 
 
+@pytest.mark.parametrize("optimizer", ["sv2n", "muon"])
+def test_no_collection_while_capturing(dev, optimizer):
+    """A graph among the garbage, collected while another is captured, ends the process
+    (its destructor synchronises the device): the collector is off meanwhile, and on
+    again afterwards."""
+    import gc
+    from spotv2net_amd import synthetic_batch
+    from spotv2net_amd.train import ForwardStep, TrainStep
+    model, _ = build(dev, hidden=(7, 5), heads=3, seed=2)
+    data = synthetic_batch(2, 2, seed=0, device=dev)
+    seen = []
+
+    def prepare():
+        if torch.cuda.is_current_stream_capturing():
+            seen.append(gc.isenabled())
+
+    TrainStep(model, data, optimizer=optimizer, prepare=prepare)
+    ForwardStep(model.eval(), data, prepare=prepare)
+    assert seen == [False, False] and gc.isenabled()
+
+
 def test_flat_layout(dev):
     """Every parameter starts on 16 bytes, the matrices last, values kept."""
     from spotv2net_amd import synthetic_batch

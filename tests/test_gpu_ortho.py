@@ -13,6 +13,8 @@ import math
 import pytest
 import torch
 
+from spotv2net_amd.graphed import _no_gc
+
 pytestmark = pytest.mark.gpu
 
 NS = (3.4445, -4.7750, 2.0315)
@@ -359,7 +361,7 @@ def test_replayed_graphs(dev):
     graphs = []
     for _ in range(2):
         g = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(g):
+        with _no_gc(), torch.cuda.graph(g):
             out = step(ws, ms)
         graphs.append((g, out))
     for k in range(6):
@@ -461,7 +463,7 @@ def test_captured_large_products(dev):
         muon_step([w.clone() for w in ws], gs, [m.clone() for m in ms], lr=0.02)
     torch.cuda.current_stream().wait_stream(s)
     graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph):
+    with _no_gc(), torch.cuda.graph(graph):
         muon_step(ws, gs, ms, lr=0.02)
     for k in range(3):
         for i, g in enumerate(gs):
