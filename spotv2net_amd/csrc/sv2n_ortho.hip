@@ -448,14 +448,11 @@ __device__ __forceinline__ f32x16 ns_mfma_exact(const f16x8* a, const f16x8* b, 
   return c;
 }
 
-// The three (or, PR = 1, one) f16 products of a pair of fragments
-template <int PR>
+// The three f16 products of a pair of fragments
 __device__ __forceinline__ f32x16 ns_mfma(const f16x8* a, const f16x8* b, f32x16 c) {
   c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], b[0], c, 0, 0, 0);
-  if (PR == 3) {
-    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], b[1], c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1], b[0], c, 0, 0, 0);
-  }
+  c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], b[1], c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1], b[0], c, 0, 0, 0);
   return c;
 }
 
@@ -476,13 +473,12 @@ __device__ __forceinline__ f32x16 ns_mfma(const f16x8* a, const f16x8* b, f32x16
 // FT = 4 keeps 256 accumulators and two steps of fragments in the 512 registers of the
 // one wave per SIMD.  big0 >= 0 (FT = 2): the blocks are quarters of the 128 x 128 tiles
 // from big0 on, what whole rounds of FT = 4 left.
-template <int EPI, int FT, int W, int PR>
+template <int EPI, int FT, int W>
 __global__ __launch_bounds__(64 * W, FT == 4 ? 1 : 2) void k_ns_mm(NsArgs A, NsScale sc, int cur, int big0) {
   // (deeper does not help: 2 to 5 steps measure the same.  FT = 1 and 2 are bound by the
   // 64 B a cycle that a CU's L1 hands its registers: with every load a hit they take 80 %
   // of the time, and without the products 90 to 100 %)
-  constexpr int DEPTH = FT == 4 ? (PR == 3 ? 2 : 4) : FT == 2 ? 2 : 4;
-  constexpr int PL = PR == 3 ? 2 : 1;
+  constexpr int DEPTH = FT == 1 ? 4 : 2;
   constexpr int TB = 32 * FT;
   extern __shared__ float s_sum[];
   const int bx = ns_xcd(blockIdx.x, gridDim.x);
@@ -519,7 +515,7 @@ __global__ __launch_bounds__(64 * W, FT == 4 ? 1 : 2) void k_ns_mm(NsArgs A, NsS
 #pragma unroll
     for (int x = 0; x < FT; ++x)
 #pragma unroll
-      for (int p = 0; p < PL; ++p) {
+      for (int p = 0; p < 2; ++p) {
         a[d][x][p] = *(const f16x8*)(gp + x * rg + (int64_t)k * 1024 + p * 512);
         b[d][x][p] = *(const f16x8*)(gr + x * rg + (int64_t)k * 1024 + p * 512);
       }
@@ -551,8 +547,8 @@ __global__ __launch_bounds__(64 * W, FT == 4 ? 1 : 2) void k_ns_mm(NsArgs A, NsS
     for (int d = 0; d < DEPTH - 1; ++d)
       if (k + d * W < nk) mul(d);
   };
-  auto f16 = [](const f16x8* p, const f16x8* q, f32x16 c) { return ns_mfma<PR>(p, q, c); };
-  if constexpr (FT == 1 && PR == 3) {
+  auto f16 = [](const f16x8* p, const f16x8* q, f32x16 c) { return ns_mfma(p, q, c); };
+  if constexpr (FT == 1) {
     if (M.exact) run([](const f16x8* p, const f16x8* q, f32x16 c) { return ns_mfma_exact(p, q, c); });
     else run(f16);
   } else {
@@ -658,9 +654,8 @@ __global__ __launch_bounds__(64 * W, FT == 4 ? 1 : 2) void k_ns_mm(NsArgs A, NsS
 // Q.  128 x 1,024: 4.3 + 4.5 us in two launches, 7.9 in one (92 -> 81 us with all steps).
 // Eight waves: first Q's m / 32 tiles times
 // slices of their depth, then 16 K values of X's product each.
-template <int EPI, int PR>
+template <int EPI>
 __global__ __launch_bounds__(512, 2) void k_ns_qx(NsArgs A, NsScale sc, int cur) {
-  constexpr int PL = PR == 3 ? 2 : 1;
   __shared__ __attribute__((aligned(16))) float sum[8][16][64];
   __shared__ __attribute__((aligned(16))) _Float16 qf[8][2][512];
   const NsTile tl = ns_tile_of<32, EPI>(A, ns_xcd(blockIdx.x, gridDim.x));
@@ -672,13 +667,13 @@ __global__ __launch_bounds__(512, 2) void k_ns_qx(NsArgs A, NsScale sc, int cur)
   const int tiles = kp / 32, slices = 8 / tiles;
   const int tq = wave % tiles, sl = wave / tiles;
   auto product = [&](const f16x8* p, const f16x8* q, f32x16 c) {
-    if (PR == 3 && M.exact) return ns_mfma_exact(p, q, c);
-    return ns_mfma<PR>(p, q, c);
+    if (M.exact) return ns_mfma_exact(p, q, c);
+    return ns_mfma(p, q, c);
   };
   // X's fragment of this wave's K values, in flight meanwhile
   f16x8 xb[2];
 #pragma unroll
-  for (int p = 0; p < PL; ++p)
+  for (int p = 0; p < 2; ++p)
     xb[p] = *(const f16x8*)(R + ns_blk(tl.tj, min(wave, nk - 1), kp) + p * 512 + lane * 8);
   f32x16 acc;
 #pragma unroll
@@ -686,7 +681,7 @@ __global__ __launch_bounds__(512, 2) void k_ns_qx(NsArgs A, NsScale sc, int cur)
   for (int k = sl; k < nk; k += slices) {
     f16x8 a[2], b[2];
 #pragma unroll
-    for (int p = 0; p < PL; ++p) {
+    for (int p = 0; p < 2; ++p) {
       a[p] = *(const f16x8*)(S + ns_blk(tq, k, kp) + p * 512 + lane * 8);
       b[p] = *(const f16x8*)(S + ns_blk(tl.ti, k, kp) + p * 512 + lane * 8);
     }
@@ -1050,11 +1045,11 @@ static int64_t ns_count(NsArgs& A, int tile, F&& takes) {
   });
 }
 
-template <int EPI, int FT, int W, int PR>
+template <int EPI, int FT, int W>
 static void ns_launch(NsArgs& A, const NsScale& sc, int cur, int64_t blocks, int big0,
                       hipStream_t stream) {
   constexpr int lds = FT == 4 ? 131072 : FT == 2 ? 32768 : W * 4096;
-  auto* k = k_ns_mm<EPI, FT, W, PR>;
+  auto* k = k_ns_mm<EPI, FT, W>;
   if (lds > 65536)
     (void)hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(64 * W), lds, stream, A, sc, cur, big0);
@@ -1065,13 +1060,13 @@ static void ns_launch(NsArgs& A, const NsScale& sc, int cur, int64_t blocks, int
 // tiles of 64, as do products that never have so many; tiles of 32 where even those
 // are under NS_TINY (the measured sides: k_ns_mm).  Exact matrices run on tiles of 32,
 // in a launch of their own where the others have larger ones.
-template <int EPI, int PR>
+template <int EPI>
 static void ns_product(NsArgs& A, const NsScale& sc, int cur, int pad, hipStream_t stream) {
   auto all = [](const NsMat&) { return true; };
   auto exact = [](const NsMat& M) { return M.exact != 0; };
   auto split = [](const NsMat& M) { return M.exact == 0; };
   if (ns_count<EPI>(A, 64, split) < NS_TINY) {
-    ns_launch<EPI, 1, 8, PR>(A, sc, cur, ns_count<EPI>(A, 32, all), -1, stream);
+    ns_launch<EPI, 1, 8>(A, sc, cur, ns_count<EPI>(A, 32, all), -1, stream);
     return;
   }
   int64_t big = 0;
@@ -1080,13 +1075,13 @@ static void ns_product(NsArgs& A, const NsScale& sc, int cur, int pad, hipStream
     big = n / 256 * 256;
     if (n - big >= NS_HALF) big = n;
     if (big > 0) {
-      ns_launch<EPI, 4, 4, PR>(A, sc, cur, big, -1, stream);
-      if (n > big) ns_launch<EPI, 2, 4, PR>(A, sc, cur, 4 * (n - big), (int)big, stream);
+      ns_launch<EPI, 4, 4>(A, sc, cur, big, -1, stream);
+      if (n > big) ns_launch<EPI, 2, 4>(A, sc, cur, 4 * (n - big), (int)big, stream);
     }
   }
-  if (big == 0) ns_launch<EPI, 2, 4, PR>(A, sc, cur, ns_count<EPI>(A, 64, split), -1, stream);
+  if (big == 0) ns_launch<EPI, 2, 4>(A, sc, cur, ns_count<EPI>(A, 64, split), -1, stream);
   const int64_t small = ns_count<EPI>(A, 32, exact);
-  if (small > 0) ns_launch<EPI, 1, 8, PR>(A, sc, cur, small, -1, stream);
+  if (small > 0) ns_launch<EPI, 1, 8>(A, sc, cur, small, -1, stream);
 }
 
 // Whether Q and X's product go in one launch: every matrix small enough for k_ns_qx, and
@@ -1097,35 +1092,21 @@ static bool ns_fused(NsArgs& A) {
   return ns_count<NS_X>(A, 32, [](const NsMat&) { return true; }) <= NS_FUSED;
 }
 
-template <int PR>
 static void ns_one_step(NsArgs& A, const NsScale& sc, int s, bool last, int pad,
                         hipStream_t stream) {
   const int cur = s & 1;
-  ns_product<NS_S, PR>(A, sc, cur, pad, stream);
+  ns_product<NS_S>(A, sc, cur, pad, stream);
   if (ns_fused(A)) {
     const int64_t n = ns_count<NS_X>(A, 32, [](const NsMat&) { return true; });
     if (!last)
-      hipLaunchKernelGGL((k_ns_qx<NS_X, PR>), dim3((unsigned)n), dim3(512), 0, stream, A, sc, cur);
-    else if constexpr (PR == 3)  // (the last step keeps both planes)
-      hipLaunchKernelGGL((k_ns_qx<NS_LAST, PR>), dim3((unsigned)n), dim3(512), 0, stream, A, sc,
-                         cur);
+      hipLaunchKernelGGL(k_ns_qx<NS_X>, dim3((unsigned)n), dim3(512), 0, stream, A, sc, cur);
+    else
+      hipLaunchKernelGGL(k_ns_qx<NS_LAST>, dim3((unsigned)n), dim3(512), 0, stream, A, sc, cur);
     return;
   }
-  ns_product<NS_Q, PR>(A, sc, cur, pad, stream);
-  if (!last) ns_product<NS_X, PR>(A, sc, cur, pad, stream);
-  else if constexpr (PR == 3) ns_product<NS_LAST, PR>(A, sc, cur, pad, stream);
-}
-
-// Steps at the start that may use the hi planes alone, where the result is bf16: with
-// |X|_F = 1 the singular values of an m-row matrix are about 1/sqrt(m), so S and Q are
-// a small correction to a X there (which keeps both planes) and their 2^-12 roundings
-// stay far below the result's 2^-9.  Measured against 64 bits (random, low-rank and
-// gradient-like matrices): the bf16 result's error grows by 0-1 % with 2 such steps
-// from m = 128 and by 0-5 % with 3 from m = 1,024; 16-row matrices would lose 27 %.
-static int ns_cheap(const NsMat& M, const NsScale& sc, int steps) {
-  if (M.dtype != SV2N_DT_BF16 || std::fabs(sc.a) > 4.f) return 0;
-  const int h = M.m >= 1024 ? 3 : M.m >= 128 ? 2 : 0;
-  return std::max(0, std::min(h, steps - 2));
+  ns_product<NS_Q>(A, sc, cur, pad, stream);
+  if (!last) ns_product<NS_X>(A, sc, cur, pad, stream);
+  else ns_product<NS_LAST>(A, sc, cur, pad, stream);
 }
 
 template <typename T>
@@ -1155,11 +1136,7 @@ static void ns_run_as(NsArgs& A, const NsScale& sc, int steps, int pad, hipStrea
   if (!B.count) return;
   n = ns_blocks(B, [](const NsMat& M) -> int64_t { return (int64_t)(M.mp / 64) * (M.np / 64); });
   hipLaunchKernelGGL(k_ns_split<T>, dim3((unsigned)n), dim3(256), 0, stream, B, sc);
-  const int cheap = ns_cheap(B.mat[0], sc, steps);  // (16-bit types come one matrix a call)
-  for (int k = 0; k < steps; ++k) {
-    if (k < cheap) ns_one_step<1>(B, sc, k, false, pad, stream);
-    else ns_one_step<3>(B, sc, k, k + 1 == steps, pad, stream);
-  }
+  for (int k = 0; k < steps; ++k) ns_one_step(B, sc, k, k + 1 == steps, pad, stream);
 }
 
 static int ns_run(NsArgs& A, const NsScale& sc, int steps, int pad, hipStream_t stream) {
