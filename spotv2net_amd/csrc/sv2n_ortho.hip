@@ -11,12 +11,18 @@
 // (22 bits; what the scale leaves below f16's range is under 2^-38 of the bound).
 // A product keeps hi·hi + hi·lo + lo·hi in f32 accumulators: three f16 products
 // at 1/3 of that peak each, where an exact f32 product has 1/16 of it.  Against
-// 64 bits the result is as close as one of f32 products (the steps amplify any
-// rounding of the input by up to a^steps, so fewer bits are not enough for f32).
+// 64 bits the result as a whole is as close as one of f32 products (the steps amplify
+// any rounding of the input by up to a^steps, so fewer bits are not enough for f32).
 //
-// (Where the smaller side is at most 32 the sums are so short that those 22 bits would
-// be the largest error, up to 3.6 times that of f32 products; the work there is next to
-// nothing, so the operands are f32 and the products v_mfma_f32_32x32x2_f32.)
+// Two cases take f32 operands and v_mfma_f32_32x32x2_f32 instead:
+// - The smaller side is at most 32: the sums are so short that those 22 bits would be
+//   the largest error, up to 3.6 times that of f32 products, and the work is next to
+//   nothing.
+// - What the pairs leave out could become a visible part of the result (ns_pairs_ok):
+//   rows or columns far below the others under many steps (64 x 128, half of the rows
+//   times 1e-8, 16 steps: 3.6e-3 off in pairs, 2.7e-6 in f32), or coefficients that
+//   shrink X.  A step takes 1.1 (128 x 1,024), 1.8 (777 x 1,537) to 4.0 (4,096²) times
+//   as long as on pairs.
 //
 // S and S S are symmetric: only tiles on and below the diagonal are computed and
 // each is stored twice.  Every operand is stored with its K dimension contiguous
@@ -48,7 +54,7 @@ constexpr int NS_MAX = 16;      // matrices of one launch
 constexpr int NS_PARTS = 1024;  // most partial sums of squares of one matrix
 constexpr int NS_PART_ELEMS = 4096;
 constexpr int NS_THIN_COLS = 128;  // columns of a thin matrix a block keeps
-constexpr int NS_EXACT = 32;    // smaller sides up to which the products are f32
+constexpr int NS_EXACT = 32;    // smaller sides up to which the products are always f32
 constexpr int NS_THIN_LONG = 2048;  // length from which a thin matrix has launches of its own
 constexpr int NS_HALF = 128;    // tiles of 128 that are worth a round of their own
 constexpr int NS_FUSED = 512;   // tiles of 32 up to which blocks make their own rows of Q
@@ -63,7 +69,7 @@ struct NsMat {
   int m, n, mp, np;     // m <= n, padded to the tile
   int batch, flip;      // flip: X = Gt
   int dtype;
-  int exact;            // f32 operands and products (m <= NS_EXACT)
+  int exact;            // f32 operands and products
   int parts, part_elems; // partial sums of squares per matrix, elements of each
   float lr;             // the update's factor (with buf)
   _Float16 *x, *xt[2], *s, *q;
@@ -552,7 +558,7 @@ __global__ __launch_bounds__(64 * W, FT == 4 ? 1 : 2) void k_ns_mm(NsArgs A, NsS
     if (M.exact) run([](const f16x8* p, const f16x8* q, f32x16 c) { return ns_mfma_exact(p, q, c); });
     else run(f16);
   } else {
-    run(f16);  // (exact matrices come on FT = 1 alone)
+    run(f16);  // (f32 operands come on FT = 1 alone)
   }
   if constexpr (FT == 4) {
     // wave w finishes the 64 x 64 quadrant (w / 2, w % 2); two quadrants' sums at a
@@ -902,40 +908,76 @@ __global__ __launch_bounds__(256) void k_ns_thin(NsArgs A, NsScale sc, int cur, 
 // ---------------------------------------------------------------------------
 static inline int64_t ns_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 
-// Largest |f| of f(x) = x·p(x²) and of q(λ) = b λ + c λ² over [0, hi]: both are
-// smooth, so a grid and the polynomials' own stationary points settle it.
-static void ns_bounds(double a, double b, double c, double hi, double* f_max, double* q_max) {
-  auto f = [&](double x) { return std::fabs(x * (a + b * x * x + c * x * x * x * x)); };
-  auto q = [&](double l) { return std::fabs(b * l + c * l * l); };
-  double fm = f(hi), qm = q(hi * hi);
-  // f' = a + 3 b y + 5 c y² at y = x²
-  const double dis = 9 * b * b - 20 * a * c;
+// What one step does to singular values in [0, hi], f(x) = x·p(x²), p(y) = a + b y + c y²:
+// the largest |f|; of q(y) = b y + c y² the largest |q|; the largest |p| or |f'|, which is
+// how far the step can multiply an error of X; and the least |f| over [lo, hi].  All are
+// smooth, so the ends and the polynomials' own stationary points settle it.
+struct NsStep {
+  double f_max, q_max, gain, f_min;
+};
+static NsStep ns_step(double a, double b, double c, double lo, double hi) {
+  auto f = [&](double x) { return x * (a + b * x * x + c * x * x * x * x); };
+  auto q = [&](double y) { return std::fabs(b * y + c * y * y); };
+  auto p = [&](double y) { return std::fabs(a + b * y + c * y * y); };
+  auto fd = [&](double y) { return std::fabs(a + 3 * b * y + 5 * c * y * y); };
+  const double top = hi * hi;
+  // inside (0, top): where q and p (one shape), f' and f turn
+  double turn_p = -1.0, turn_fd = -1.0, turn_f[2] = {-1.0, -1.0};
   if (c != 0.0) {
-    if (dis >= 0.0)
-      for (double s : {-1.0, 1.0}) {
-        const double y = (-3 * b + s * std::sqrt(dis)) / (10 * c);
-        if (y > 0.0 && y < hi * hi) fm = std::max(fm, f(std::sqrt(y)));
-      }
-    const double l = -b / (2 * c);
-    if (l > 0.0 && l < hi * hi) qm = std::max(qm, q(l));
+    turn_p = -b / (2 * c);
+    turn_fd = -3 * b / (10 * c);
+    const double dis = 9 * b * b - 20 * a * c;  // of f' = a + 3 b y + 5 c y²
+    if (dis >= 0.0) {
+      turn_f[0] = (-3 * b - std::sqrt(dis)) / (10 * c);
+      turn_f[1] = (-3 * b + std::sqrt(dis)) / (10 * c);
+    }
   } else if (b != 0.0) {
-    const double y = -a / (3 * b);
-    if (y > 0.0 && y < hi * hi) fm = std::max(fm, f(std::sqrt(y)));
+    turn_f[0] = -a / (3 * b);
   }
-  *f_max = fm;
-  *q_max = qm;
+  auto in = [&](double y) { return y > 0.0 && y < top; };
+  NsStep r;
+  r.f_max = std::fabs(f(hi));
+  r.q_max = q(top);
+  r.gain = std::max(std::max(p(0.0), p(top)), fd(top));
+  if (in(turn_p)) {
+    r.q_max = std::max(r.q_max, q(turn_p));
+    r.gain = std::max(r.gain, p(turn_p));
+  }
+  if (in(turn_fd)) r.gain = std::max(r.gain, fd(turn_fd));
+  double least = std::min(f(lo), f(hi)), most = std::max(f(lo), f(hi));
+  for (double y : turn_f)
+    if (in(y)) {
+      const double x = std::sqrt(y), v = f(x);
+      r.f_max = std::max(r.f_max, std::fabs(v));
+      if (x > lo) {
+        least = std::min(least, v);
+        most = std::max(most, v);
+      }
+    }
+  r.f_min = least > 0.0 ? least : most < 0.0 ? -most : 0.0;
+  return r;
 }
+
+// What the steps can do to X: `gain` to an error of it, `least` its smallest norm
+struct NsRange {
+  double gain, least;
+};
 
 // The power-of-two scales of X, S and Q from the largest singular value any step
 // can reach; false if the coefficients let them grow past 2^8.
-static bool ns_scales(int steps, NsScale* sc) {
-  double top = 1.0, hi = 1.0, qm = 0.0;
+static bool ns_scales(int steps, NsScale* sc, NsRange* range) {
+  // (the largest singular value of an m-row X_0 is at least 1/sqrt(m))
+  double top = 1.0, hi = 1.0, lo = 1.0 / 128, qm = 0.0;
+  static_assert(SV2N_NS_MAX_SIDE == 128 * 128, "lo");
+  *range = {1.0, lo};
   for (int k = 0; k < steps; ++k) {
-    double f, q;
-    ns_bounds(sc->a, sc->b, sc->c, hi, &f, &q);
-    qm = std::max(qm, q);
-    top = std::max(top, f);
-    hi = f;
+    const NsStep r = ns_step(sc->a, sc->b, sc->c, lo, hi);
+    qm = std::max(qm, r.q_max);
+    top = std::max(top, r.f_max);
+    hi = r.f_max;
+    lo = r.f_min;
+    range->gain *= std::max(1.0, r.gain);
+    range->least = std::min(range->least, lo);
     if (!(top <= 256.0) || !(qm <= 65536.0)) return false;
     if (hi == 0.0) break;
   }
@@ -950,11 +992,21 @@ static bool ns_scales(int steps, NsScale* sc) {
   return true;
 }
 
+// Whether pairs of f16 are as good as f32 for a matrix under these steps.  An entry held
+// as a pair is off by up to 2^-39 (0.3 of it on average) however small it is, which f32
+// is not.  Over the matrix that is 2^-41 sqrt(rows·cols) in the 2-norm, and the steps
+// multiply it by at most `gain`: allowed up to 2^-17 of a result whose norm is near 1 or
+// more.  (The default coefficients: five steps at every size, 6 to 4,096², 8 to 64 x 128.)
+// And X must not shrink by more than 16, or 2^-39 comes nearer to its own entries.
+static bool ns_pairs_ok(const NsMat& M, const NsRange& range) {
+  return range.gain * std::sqrt((double)M.rows * M.cols) <= 16777216.0 &&
+         range.least >= 1.0 / 2048;
+}
+
 static void ns_shape(NsMat* M) {
   M->flip = M->rows > M->cols;
   M->m = std::min(M->rows, M->cols);
   M->n = std::max(M->rows, M->cols);
-  M->exact = M->m <= NS_EXACT;
   const int64_t total = (int64_t)M->rows * M->cols;
   const int64_t each = std::max<int64_t>(NS_PART_ELEMS, (total + NS_PARTS - 1) / NS_PARTS);
   M->part_elems = (int)ns_up(each, 8);
@@ -974,13 +1026,13 @@ static int ns_pad(const NsMat* mats, int count) {
 }
 
 // Whether a group's matrices of m <= NS_EXACT go to k_ns_thin: always where the others
-// (if any) take tiles above 32 or one is longer than NS_THIN_LONG; beside small matrices
-// they ride in those launches as exact tiles instead of adding their own.
+// (if any) have NS_TINY tiles of 64 or one is longer than NS_THIN_LONG; beside small
+// matrices they ride in those launches as exact tiles instead of adding their own.
 static bool ns_thin(const NsMat* mats, int count) {
   int64_t tiles = 0;
   bool others = false, any = false, longer = false;
   for (int i = 0; i < count; ++i) {
-    if (mats[i].exact) {
+    if (mats[i].m <= NS_EXACT) {
       any = true;
       longer |= mats[i].n > NS_THIN_LONG;
     } else {
@@ -1004,7 +1056,7 @@ static int64_t ns_plan(NsMat* mats, int count, int pad, char* ws) {
   for (int i = 0; i < count; ++i) {
     NsMat& M = mats[i];
     M.thin = nullptr;
-    if (thin && M.exact) {
+    if (thin && M.m <= NS_EXACT) {
       M.mp = NS_EXACT;
       M.np = (int)ns_up(M.n, NS_THIN_COLS);
       M.part = (double*)take((int64_t)M.batch * M.parts * 8);
@@ -1036,12 +1088,12 @@ static int64_t ns_blocks(NsArgs& A, F&& per) {
   return n;
 }
 
-// Tiles of a product over the group's matrices that `takes` chooses
-template <int EPI, typename F>
-static int64_t ns_count(NsArgs& A, int tile, F&& takes) {
+// Tiles of a product over the group's matrices; `pairs`: over those in pairs of f16
+template <int EPI>
+static int64_t ns_count(NsArgs& A, int tile, bool pairs) {
   return ns_blocks(A, [&](const NsMat& M) -> int64_t {
     const int64_t tm = M.mp / tile, tn = M.np / tile;
-    return !takes(M) ? 0 : EPI == NS_S || EPI == NS_Q ? tm * (tm + 1) / 2 : tm * tn;
+    return pairs && M.exact ? 0 : EPI == NS_S || EPI == NS_Q ? tm * (tm + 1) / 2 : tm * tn;
   });
 }
 
@@ -1058,30 +1110,27 @@ static void ns_launch(NsArgs& A, const NsScale& sc, int cur, int64_t blocks, int
 // A product over the group's tiles.  Tiles of 128 where they fill at least half of the
 // chip's 256 CUs (one block each) in every round; fewer than that left over go on
 // tiles of 64, as do products that never have so many; tiles of 32 where even those
-// are under NS_TINY (the measured sides: k_ns_mm).  Exact matrices run on tiles of 32,
-// in a launch of their own where the others have larger ones.
+// are under NS_TINY (the measured sides: k_ns_mm), and for f32 operands, whose products
+// are the bound there already (tiles of 64, us a step: 4,096² 3,450 -> 3,780, 777 x 1,537
+// 77 -> 87, 1,024² 86 -> 62).  A group is all f32 operands, or those of m <= NS_EXACT
+// beside pairs with fewer than NS_TINY tiles (ns_thin).
 template <int EPI>
 static void ns_product(NsArgs& A, const NsScale& sc, int cur, int pad, hipStream_t stream) {
-  auto all = [](const NsMat&) { return true; };
-  auto exact = [](const NsMat& M) { return M.exact != 0; };
-  auto split = [](const NsMat& M) { return M.exact == 0; };
-  if (ns_count<EPI>(A, 64, split) < NS_TINY) {
-    ns_launch<EPI, 1, 8>(A, sc, cur, ns_count<EPI>(A, 32, all), -1, stream);
+  if (ns_count<EPI>(A, 64, true) < NS_TINY) {
+    ns_launch<EPI, 1, 8>(A, sc, cur, ns_count<EPI>(A, 32, false), -1, stream);
     return;
   }
-  int64_t big = 0;
   if (pad == 128) {
-    const int64_t n = ns_count<EPI>(A, 128, split);
-    big = n / 256 * 256;
+    const int64_t n = ns_count<EPI>(A, 128, true);
+    int64_t big = n / 256 * 256;
     if (n - big >= NS_HALF) big = n;
     if (big > 0) {
       ns_launch<EPI, 4, 4>(A, sc, cur, big, -1, stream);
       if (n > big) ns_launch<EPI, 2, 4>(A, sc, cur, 4 * (n - big), (int)big, stream);
+      return;
     }
   }
-  if (big == 0) ns_launch<EPI, 2, 4>(A, sc, cur, ns_count<EPI>(A, 64, split), -1, stream);
-  const int64_t small = ns_count<EPI>(A, 32, exact);
-  if (small > 0) ns_launch<EPI, 1, 8>(A, sc, cur, small, -1, stream);
+  ns_launch<EPI, 2, 4>(A, sc, cur, ns_count<EPI>(A, 64, true), -1, stream);
 }
 
 // Whether Q and X's product go in one launch: every matrix small enough for k_ns_qx, and
@@ -1089,7 +1138,7 @@ static void ns_product(NsArgs& A, const NsScale& sc, int cur, int pad, hipStream
 static bool ns_fused(NsArgs& A) {
   for (int i = 0; i < A.count; ++i)
     if (A.mat[i].mp > 128) return false;
-  return ns_count<NS_X>(A, 32, [](const NsMat&) { return true; }) <= NS_FUSED;
+  return ns_count<NS_X>(A, 32, false) <= NS_FUSED;
 }
 
 static void ns_one_step(NsArgs& A, const NsScale& sc, int s, bool last, int pad,
@@ -1097,7 +1146,7 @@ static void ns_one_step(NsArgs& A, const NsScale& sc, int s, bool last, int pad,
   const int cur = s & 1;
   ns_product<NS_S>(A, sc, cur, pad, stream);
   if (ns_fused(A)) {
-    const int64_t n = ns_count<NS_X>(A, 32, [](const NsMat&) { return true; });
+    const int64_t n = ns_count<NS_X>(A, 32, false);
     if (!last)
       hipLaunchKernelGGL(k_ns_qx<NS_X>, dim3((unsigned)n), dim3(512), 0, stream, A, sc, cur);
     else
@@ -1137,6 +1186,14 @@ static void ns_run_as(NsArgs& A, const NsScale& sc, int steps, int pad, hipStrea
   n = ns_blocks(B, [](const NsMat& M) -> int64_t { return (int64_t)(M.mp / 64) * (M.np / 64); });
   hipLaunchKernelGGL(k_ns_split<T>, dim3((unsigned)n), dim3(256), 0, stream, B, sc);
   for (int k = 0; k < steps; ++k) ns_one_step(B, sc, k, k + 1 == steps, pad, stream);
+}
+
+// Which products a group takes: one matrix that needs f32 operands takes the group along
+// (a step's launches are shared), else those of m <= NS_EXACT have them alone
+static void ns_exact(NsArgs* A, const NsRange& range) {
+  bool all = false;
+  for (int i = 0; i < A->count; ++i) all |= !ns_pairs_ok(A->mat[i], range);
+  for (int i = 0; i < A->count; ++i) A->mat[i].exact = all || A->mat[i].m <= NS_EXACT;
 }
 
 static int ns_run(NsArgs& A, const NsScale& sc, int steps, int pad, hipStream_t stream) {
@@ -1182,12 +1239,14 @@ extern "C" int sv2n_orthogonalize(const void* g, int64_t ld, int64_t batch_strid
   NsArgs A{};
   NsScale sc{};
   sc.a = a; sc.b = b; sc.c = c; sc.eps = eps;
-  if (!ns_scales(steps, &sc)) return SV2N_ERR_ARG;
+  NsRange range;
+  if (!ns_scales(steps, &sc, &range)) return SV2N_ERR_ARG;
   NsMat& M = A.mat[0];
   A.count = 1;
   M.g = g; M.ld = ld; M.g_batch = batch_stride; M.out = out; M.dtype = dtype;
   M.rows = (int)rows; M.cols = (int)cols; M.batch = (int)batch;
   ns_shape(&M);
+  ns_exact(&A, range);
   const int pad = ns_pad(&M, 1);
   if (!workspace || workspace_bytes < ns_plan(&M, 1, pad, nullptr)) return SV2N_ERR_WORKSPACE;
   if ((uintptr_t)workspace & 255) return SV2N_ERR_ALIGN;
@@ -1249,7 +1308,8 @@ extern "C" int sv2n_muon_step(const sv2n_muon_matrix* mats, int count, double lr
   sc.fresh = (float)(1.0 - momentum);
   sc.nesterov = nesterov != 0;
   sc.keep = (float)(1.0 - lr * weight_decay);
-  if (!ns_scales(steps, &sc)) return SV2N_ERR_ARG;
+  NsRange range;
+  if (!ns_scales(steps, &sc, &range)) return SV2N_ERR_ARG;
   if (!workspace || workspace_bytes < sv2n_muon_step_workspace(mats, count))
     return SV2N_ERR_WORKSPACE;
   if ((uintptr_t)workspace & 255) return SV2N_ERR_ALIGN;
@@ -1257,6 +1317,7 @@ extern "C" int sv2n_muon_step(const sv2n_muon_matrix* mats, int count, double lr
     const int n = std::min(NS_MAX, count - k);
     NsArgs A{};
     ns_group(mats + k, n, lr, &A);
+    ns_exact(&A, range);
     const int pad = ns_pad(A.mat, n);
     ns_plan(A.mat, n, pad, (char*)workspace);
     const int rc = ns_run(A, sc, steps, pad, stream);
