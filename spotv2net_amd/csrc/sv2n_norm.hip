@@ -5,11 +5,13 @@
 //
 // Both passes are bound by memory: the forward reads x once and writes y, the
 // backward reads x and dy once and writes dx.  A row is held in the registers
-// of TPR threads (16 B per thread and load), so the two-step variance (mean
-// first, then the squared deviations) costs no second read and loses nothing to
-// cancellation.  TPR is the smallest group that leaves a thread at most 16
-// elements (32 past rows of 8,192), since the backward holds five such arrays (x, dy, w and the sums of
-// dw and db): 16 threads for a row of 128, so a wave carries four of them.
+// of TPR threads (16 B per thread and load), so taking the mean, then the mean of the
+// deviations from it (added to the mean), then the squares of those left costs no second
+// read and loses nothing to cancellation: a row of equal values has exactly that mean,
+// z = 0 and variance 0, where a mean off by its rounding would come out scaled by rstd,
+// up to 1/sqrt(eps).  TPR is the smallest group that leaves a thread at most 16 elements
+// (32 past rows of 8,192), since the backward holds five such arrays (x, dy, w and the
+// sums of dw and db): 16 threads for a row of 128, so a wave carries four of them.
 // Groups walk the rows with a stride; each thread owns the same columns in every
 // row, so dw and db are summed in its registers (f32) and leave the block once,
 // as a partial per block that a second launch adds in block order: no atomics,
@@ -228,17 +230,21 @@ __global__ __launch_bounds__(ln_threads<TPR>()) void k_ln_fwd(
       }
     fetch(row + step);
     s = group_sum<G>(s);
-    float m, m2 = 0.f;
-    if constexpr (WPR <= 1) {
-      m = s * inv_c;
-    } else {
-      // the wave's own mean first; the waves are merged below
+    float m, m1 = 0.f, m2 = 0.f;
+    int n = cols;  // elements of the group, or (rows of several waves) of the wave
+    if constexpr (WPR > 1) {
       const int wv0 = (t / 64) * 64 * V;
-      int n = 0;
+      n = 0;
 #pragma unroll
       for (int k = 0; k < NPT; ++k) n += max(0, min(64 * V, cols - k * TPR * V - wv0));
-      m = n > 0 ? s / (float)n : 0.f;
     }
+    const float fn = (float)max(n, 1);
+    m = s / fn;
+#pragma unroll
+    for (int k = 0; k < NPT; ++k)
+#pragma unroll
+      for (int j = 0; j < V; ++j) m1 += k < NPT - 1 || at[k].has(j) ? v[k][j] - m : 0.f;
+    m += group_sum<G>(m1) / fn;
 #pragma unroll
     for (int k = 0; k < NPT; ++k)
 #pragma unroll
@@ -248,23 +254,24 @@ __global__ __launch_bounds__(ln_threads<TPR>()) void k_ln_fwd(
       }
     m2 = group_sum<G>(m2);
     if constexpr (WPR > 1) {
-      // one exchange per row (two buffers, so one barrier): the mean of the
-      // means by their counts, and Σ m2 + n·(mean_wave - mean)²
+      // one exchange per row (two buffers, so one barrier): the mean of the waves'
+      // means by their counts, from the first one's, and Σ m2 + n·(mean_wave - mean)²
       float(*mine)[2] = red[buf] + grp * WPR;
       if ((t & 63) == 0) {
         mine[t / 64][0] = m;
         mine[t / 64][1] = m2;
       }
       __syncthreads();
+      const float m0 = mine[0][0];
       float tot = 0.f, q = 0.f;
 #pragma unroll
       for (int u = 0; u < WPR; ++u) {
         int n = 0;
 #pragma unroll
         for (int k = 0; k < NPT; ++k) n += max(0, min(64 * V, cols - k * TPR * V - u * 64 * V));
-        tot = fmaf((float)n, mine[u][0], tot);
+        tot = fmaf((float)n, mine[u][0] - m0, tot);
       }
-      m = tot * inv_c;
+      m = m0 + tot / (float)cols;
 #pragma unroll
       for (int u = 0; u < WPR; ++u) {
         int n = 0;
