@@ -891,8 +891,9 @@ def gat_stack(x: torch.Tensor, edge_attr: Optional[torch.Tensor], convs: Sequenc
         # the gradients go straight to p.grad: an empty leaf stands for the parameters,
         # so that the node has no edge to their accumulation nodes (an eager graph that
         # is alive keeps those on its own stream, and a captured backward would wait for
-        # that stream)
-        params = [torch.empty(0, device=x.device, requires_grad=True)]
+        # that stream); it trains where one of them does
+        params = [torch.empty(0, device=x.device,
+                              requires_grad=any(p.requires_grad for p in params))]
     out = _GATStack.apply(x, edge_attr, tuple(convs), layout, int(act), float(post_dropout),
                           bool(training), precision, x_bf16,
                           None if norms is None else tuple(norms), *params)

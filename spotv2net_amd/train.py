@@ -325,14 +325,16 @@ class TrainStep:
                 res = head_mse_train_split(h, self.model.linear, sh.data.y_x, self.loss_sum)
                 if res is not None:
                     loss, dh, finish = res
-                    torch.autograd.backward(h, dh)
+                    if h.requires_grad:  # else every layer is frozen
+                        torch.autograd.backward(h, dh)
                     finish()
                     sh.loss = loss.detach()
                     return
                 res = head_mse_train(h, self.model.linear, sh.data.y_x, self.loss_sum)
                 if res is not None:
                     loss, dh = res
-                    torch.autograd.backward(h, dh)
+                    if h.requires_grad:
+                        torch.autograd.backward(h, dh)
                     sh.loss = loss.detach()
                     return
                 loss = self.model.mse_loss(sh.data)
