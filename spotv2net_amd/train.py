@@ -208,6 +208,14 @@ def make_adam(params, lr: float):
         return torch.optim.Adam(params, lr=lr, capturable=True, foreach=True)
 
 
+OPTIMIZERS = ("sv2n", "muon", "torch")
+
+
+def _check_optimizer(name) -> None:
+    if name not in OPTIMIZERS:
+        raise ValueError(f"optimizer is one of {OPTIMIZERS}, got {name!r}")
+
+
 class _Shape:
     """One captured batch shape of a TrainStep: its static data, the optional
     capturable ``prepare`` (e.g. WindowDataset.fill from an index buffer),
@@ -233,7 +241,8 @@ class TrainStep:
     undone (parameters, buffers, optimizer state, RNG).
 
     ``optimizer``: "sv2n" (Adam over the flat buffers, one launch), "muon" (Muon for
-    the weight matrices, Adam for the rest: ``FlatMuon``), else torch's Adam.
+    the weight matrices with momentum 0.95, Nesterov's rule and no weight decay, Adam
+    for the rest: ``FlatMuon``) or "torch" (torch's Adam).
 
     ``loss_sum``: a device scalar every step adds its loss to inside the
     captured step (the reference's per-epoch running loss,
@@ -245,6 +254,7 @@ class TrainStep:
                  prepare: Optional[Callable[[], None]] = None,
                  loss_sum: Optional[torch.Tensor] = None, device_rng: bool = True,
                  dropout_seed: Optional[int] = None):
+        _check_optimizer(optimizer)
         self.model = model
         self.loss_sum = loss_sum
         self.loss_fn = loss_fn
@@ -525,6 +535,7 @@ class Fit:
                  split: float = 0.8, generator: Optional[torch.Generator] = None,
                  use_graph: bool = True, optimizer: str = "sv2n",
                  step_hook: Optional[Callable[[int, int], None]] = None):
+        _check_optimizer(optimizer)
         self.model, self.ds, self.bs = model, dataset, int(batch_size)
         n = len(dataset)
         self.n_train = int(split * n)
