@@ -241,14 +241,16 @@ struct LayerNormBackward : torch::autograd::Node {
     TORCH_CHECK(!released, torch::autograd::ERR_BACKWARD_TWICE);
     refuse_capture_from_eager();
     const bool twice = at::GradMode::is_enabled();
+    // (unpacking may run a checkpointed forward again: not below autograd)
+    const Tensor xv = x.unpack(), mv = mean.unpack(), rv = rstd.unpack();
+    const OptTensor w = has_weight ? OptTensor(weight.unpack()) : std::nullopt;
     {
       at::AutoDispatchBelowAutograd below;
-      const OptTensor w = has_weight ? OptTensor(weight.unpack()) : std::nullopt;
       const bool nx = task_should_compute_output(0);
       const bool nw = has_weight && task_should_compute_output(1);
       const bool nb = has_bias && task_should_compute_output(2);
       auto [dx, dw, db] = call_layer_norm_bwd(
-          grads[0], x.unpack(), w, mean.unpack(), rstd.unpack(), nx, nw, nb,
+          grads[0], xv, w, mv, rv, nx, nw, nb,
           has_bias ? std::optional<at::ScalarType>(bias_type) : std::nullopt);
       if (nx) out[0] = std::move(dx);
       if (nw) out[1] = std::move(dw);
