@@ -2,7 +2,7 @@
 // less than an operator implemented in Python costs to call, and an autograd node in
 // Python costs more than both passes.  Registers, for the schemas library.py defines,
 //   sv2n::layer_norm          CUDA kernel and autograd formula
-//   sv2n::layer_norm_bwd      CUDA kernel
+//   sv2n::layer_norm_bwd      CUDA kernel; not differentiable, which it says
 //   sv2n::layer_norm_bwd_acc  CUDA kernel
 // The C entries come from whichever libsv2n build the process loaded: _lib.py hands
 // their addresses to sv2n_torch_bind before the first call.
@@ -12,7 +12,6 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/library.h>
@@ -240,30 +239,19 @@ struct LayerNormBackward : torch::autograd::Node {
     if (!grads[0].defined()) return out;
     TORCH_CHECK(!released, torch::autograd::ERR_BACKWARD_TWICE);
     refuse_capture_from_eager();
-    const bool twice = at::GradMode::is_enabled();
-    // (unpacking may run a checkpointed forward again: not below autograd)
+    // (unpacking may run a checkpointed forward again, and the call is itself recorded
+    // where gradients of the gradients are: neither below autograd)
     const Tensor xv = x.unpack(), mv = mean.unpack(), rv = rstd.unpack();
     const OptTensor w = has_weight ? OptTensor(weight.unpack()) : std::nullopt;
-    {
-      at::AutoDispatchBelowAutograd below;
-      const bool nx = task_should_compute_output(0);
-      const bool nw = has_weight && task_should_compute_output(1);
-      const bool nb = has_bias && task_should_compute_output(2);
-      auto [dx, dw, db] = call_layer_norm_bwd(
-          grads[0], xv, w, mv, rv, nx, nw, nb,
-          has_bias ? std::optional<at::ScalarType>(bias_type) : std::nullopt);
-      if (nx) out[0] = std::move(dx);
-      if (nw) out[1] = std::move(dw);
-      if (nb) out[2] = std::move(db);
-    }
-    if (twice) {
-      // differentiable once: a gradient of these gradients raises
-      for (auto& t : out)
-        if (t.defined()) t = t.detach().requires_grad_(true);
-      auto err = std::make_shared<torch::autograd::DelayedError>(
-          "sv2n: layer_norm is differentiable once (its gradients have no gradient)", 3);
-      out = (*err)(std::move(out));
-    }
+    const bool nx = task_should_compute_output(0);
+    const bool nw = has_weight && task_should_compute_output(1);
+    const bool nb = has_bias && task_should_compute_output(2);
+    auto [dx, dw, db] = call_layer_norm_bwd(
+        grads[0], xv, w, mv, rv, nx, nw, nb,
+        has_bias ? std::optional<at::ScalarType>(bias_type) : std::nullopt);
+    if (nx) out[0] = std::move(dx);
+    if (nw) out[1] = std::move(dw);
+    if (nb) out[2] = std::move(db);
     return out;
   }
   void release_variables() override {
@@ -300,6 +288,39 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_autograd(const Tensor& x, const Op
   return out;
 }
 
+// What the gradients depend on, for whoever differentiates them: an error
+struct LayerNormOnce : torch::autograd::Node {
+  std::string name() const override { return "LayerNormOnce"; }
+  variable_list apply(variable_list&&) override {
+    TORCH_CHECK(false, "sv2n: layer_norm is differentiable once (its gradients have no gradient)");
+  }
+};
+
+std::tuple<Tensor, Tensor, Tensor> layer_norm_bwd_autograd(
+    const Tensor& dy, const Tensor& x, const OptTensor& weight, const Tensor& mean,
+    const Tensor& rstd, bool need_dx, bool need_dw, bool need_db,
+    std::optional<at::ScalarType> grad_dtype) {
+  const Tensor w = weight.value_or(Tensor());
+  for (const OptTensor& t : {OptTensor(dy), OptTensor(x), weight})
+    TORCH_CHECK(!torch::autograd::isFwGradDefined(t),
+                "sv2n: layer_norm is differentiable once (its gradients have no gradient)");
+  std::tuple<Tensor, Tensor, Tensor> out;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    out = call_layer_norm_bwd(dy, x, weight, mean, rstd, need_dx, need_dw, need_db, grad_dtype);
+  }
+  if (at::GradMode::is_enabled() &&
+      (dy.requires_grad() || x.requires_grad() || (w.defined() && w.requires_grad()) ||
+       mean.requires_grad() || rstd.requires_grad())) {
+    std::shared_ptr<LayerNormOnce> node(new LayerNormOnce(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(dy, x, w, mean, rstd));
+    if (need_dx) torch::autograd::set_history(std::get<0>(out), node);
+    if (need_dw) torch::autograd::set_history(std::get<1>(out), node);
+    if (need_db) torch::autograd::set_history(std::get<2>(out), node);
+  }
+  return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY_IMPL(sv2n, CUDA, m) {
@@ -307,7 +328,10 @@ TORCH_LIBRARY_IMPL(sv2n, CUDA, m) {
   m.impl("layer_norm_bwd", layer_norm_bwd);
   m.impl("layer_norm_bwd_acc", layer_norm_bwd_acc);
 }
-TORCH_LIBRARY_IMPL(sv2n, Autograd, m) { m.impl("layer_norm", layer_norm_autograd); }
+TORCH_LIBRARY_IMPL(sv2n, Autograd, m) {
+  m.impl("layer_norm", layer_norm_autograd);
+  m.impl("layer_norm_bwd", layer_norm_bwd_autograd);
+}
 
 extern "C" void sv2n_torch_bind(void* fwd, void* bwd, void* bwd_ws, void* strerror) {
   g_entries.fwd = (decltype(g_entries.fwd))fwd;
