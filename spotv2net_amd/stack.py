@@ -539,8 +539,9 @@ def stack_forward(x, edge_attr, convs, layout: GraphLayout, act: int, post_dropo
         saved_drop.append(dmask)
         xin = out
         if norms is not None:
-            xin, mean, rstd = ops.layer_norm(out, norms[l].weight, norms[l].bias, norms[l].eps)
-            saved_norm += [out, mean, rstd]
+            w = norms[l].weight
+            xin, mean, rstd = ops.layer_norm(out, w, norms[l].bias, norms[l].eps)
+            saved_norm += [out, mean, rstd, None if w is None else w.detach()]
 
     meta = _StackMeta((L, act, use_edge, hp, H, eo, fused), bf16, feid,
                       [(1.0 / (1.0 - c.dropout)) if (training and 0.0 < c.dropout < 1.0) else
@@ -571,7 +572,7 @@ def stack_backward(saved, meta: _StackMeta, convs, layout: GraphLayout, dout, ne
     waugs = sv[k:k + L]; k += L
     planes_t = sv[k:k + L]; k += L
     xb0 = sv[k]  # bf16(x) of layer 0, or None
-    normed = sv[k + 1:]  # per layer: the output before its norm, mean, rstd
+    normed = sv[k + 1:]  # per layer: the output before its norm, mean, rstd, the norm's weight
     dev = dout.device
     B, n, N = layout.num_graphs, layout.n, layout.num_nodes
 
@@ -645,8 +646,8 @@ def stack_backward(saved, meta: _StackMeta, convs, layout: GraphLayout, dout, ne
         c = convs[l]
         Hc, C = c.heads, c.out_channels
         if norms is not None:
-            dy = ops.layer_norm_bwd_acc(dy, normed[3 * l], norms[l].weight, normed[3 * l + 1],
-                                        normed[3 * l + 2], grad_of(norms[l].weight),
+            xn, mean, rstd, w = normed[4 * l:4 * l + 4]
+            dy = ops.layer_norm_bwd_acc(dy, xn, w, mean, rstd, grad_of(norms[l].weight),
                                         grad_of(norms[l].bias))
         post_u = drops[l] if meta.post_p[l] is not None else None
         if drops[l] is not None and post_u is None:
