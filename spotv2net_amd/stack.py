@@ -170,6 +170,22 @@ class _GradTargets:
         return tuple(self._views.get(i) if i in self._used else None for i in self._order)
 
 
+def _stand_in(params, device) -> torch.Tensor:
+    """The direct mode's one input for a node's parameters, whose gradients go straight
+    to ``p.grad``: an empty leaf that trains where one of them does.  The node then has
+    no edge to their accumulation nodes (an eager graph that is alive keeps those on its
+    own stream, and a captured backward would wait for that stream)."""
+    return torch.empty(0, device=device,
+                       requires_grad=any(p is not None and p.requires_grad for p in params))
+
+
+def _head_needs(ctx, linear, first: int):
+    """Which of weight and bias need a gradient (the node's inputs from ``first``)."""
+    if not ctx.direct:
+        return ctx.needs_input_grad[first:first + 2]
+    return [p is not None and p.requires_grad for p in (linear.weight, linear.bias)]
+
+
 def layer_params(conv) -> list:
     ps = [conv.lin_src.weight, conv.att_src, conv.att_dst]
     if conv.lin_edge is not None:
@@ -889,28 +905,33 @@ def gat_stack(x: torch.Tensor, edge_attr: Optional[torch.Tensor], convs: Sequenc
         if p.device != x.device:
             raise RuntimeError("parameters and data must be on the same device")
     if _direct_mode():
-        # the gradients go straight to p.grad: an empty leaf stands for the parameters,
-        # so that the node has no edge to their accumulation nodes (an eager graph that
-        # is alive keeps those on its own stream, and a captured backward would wait for
-        # that stream); it trains where one of them does
-        params = [torch.empty(0, device=x.device,
-                              requires_grad=any(p.requires_grad for p in params))]
+        params = [_stand_in(params, x.device)]
     out = _GATStack.apply(x, edge_attr, tuple(convs), layout, int(act), float(post_dropout),
                           bool(training), precision, x_bf16,
                           None if norms is None else tuple(norms), *params)
     return layout.poison(out)  # NaN if a deferred layout check failed (layout.py)
 
 
+def _head_inputs(linear: torch.nn.Linear, device):
+    """The parameters as a head node's inputs (the direct mode: their stand-in)."""
+    if _direct_mode():
+        return _stand_in((linear.weight, linear.bias), device), None
+    return linear.weight, linear.bias
+
+
 class _Head(torch.autograd.Function):
     """GATModel.linear (reference utils/models.py:120, :150) on sv2n::head_*;
-    parameter gradients are returned (or accumulated directly) like the GAT stack."""
+    parameter gradients are returned, or accumulated directly (``weight`` is then their
+    stand-in), like the GAT stack."""
 
     @staticmethod
     def forward(ctx, x, linear, weight, bias):
         x = _aligned(x)
-        out = torch.ops.sv2n.head_fwd(x, weight, bias)
         ctx.linear = linear
         ctx.direct = _direct_mode()
+        if ctx.direct:
+            weight, bias = linear.weight, linear.bias
+        out = torch.ops.sv2n.head_fwd(x, weight, bias)
         ctx.save_for_backward(x)
         return out
 
@@ -918,7 +939,7 @@ class _Head(torch.autograd.Function):
     def backward(ctx, dout):
         (x,) = ctx.saved_tensors
         lin = ctx.linear
-        grad_of = _GradTargets([lin.weight, lin.bias], ctx.needs_input_grad[2:4], ctx.direct,
+        grad_of = _GradTargets([lin.weight, lin.bias], _head_needs(ctx, lin, 2), ctx.direct,
                                x.device)
         dx = torch.ops.sv2n.head_bwd(x, lin.weight, dout, grad_of(lin.weight), grad_of(lin.bias))
         return (dx if ctx.needs_input_grad[0] else None, None) + grad_of.returned()
@@ -932,9 +953,11 @@ class _HeadMSE(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, target, linear, weight, bias, loss_sum=None):
         x = _aligned(x)
-        loss, diff = torch.ops.sv2n.head_mse_fwd(x, weight, bias, target, loss_sum)
         ctx.linear = linear
         ctx.direct = _direct_mode()
+        if ctx.direct:
+            weight, bias = linear.weight, linear.bias
+        loss, diff = torch.ops.sv2n.head_mse_fwd(x, weight, bias, target, loss_sum)
         ctx.save_for_backward(x, diff)
         return loss
 
@@ -942,7 +965,7 @@ class _HeadMSE(torch.autograd.Function):
     def backward(ctx, gloss):
         x, diff = ctx.saved_tensors
         lin = ctx.linear
-        grad_of = _GradTargets([lin.weight, lin.bias], ctx.needs_input_grad[3:5], ctx.direct,
+        grad_of = _GradTargets([lin.weight, lin.bias], _head_needs(ctx, lin, 3), ctx.direct,
                                x.device)
         dx = torch.ops.sv2n.head_mse_bwd(x, lin.weight, diff, gloss, grad_of(lin.weight),
                                          grad_of(lin.bias))
@@ -962,7 +985,8 @@ def head_mse_loss(x: torch.Tensor, linear: torch.nn.Linear, target: torch.Tensor
         if loss_sum is not None:
             loss_sum.add_(loss.detach())
         return loss
-    return _HeadMSE.apply(x, target, linear, linear.weight, linear.bias, loss_sum)
+    weight, bias = _head_inputs(linear, x.device)
+    return _HeadMSE.apply(x, target, linear, weight, bias, loss_sum)
 
 
 def head_mse_train(x: torch.Tensor, linear: torch.nn.Linear, target: torch.Tensor,
@@ -1025,4 +1049,5 @@ def linear_head(x: torch.Tensor, linear: torch.nn.Linear) -> torch.Tensor:
     _require_device(x)
     if not head_fits(linear.in_features, linear.out_features):
         return linear(x)
-    return _Head.apply(x, linear, linear.weight, linear.bias)
+    weight, bias = _head_inputs(linear, x.device)
+    return _Head.apply(x, linear, weight, bias)
