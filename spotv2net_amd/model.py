@@ -131,6 +131,11 @@ class GATModel(nn.Module):
         self.a = acts[activation]
         self._act_code = ops.ACT_CODES[activation]
 
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        if "norms" not in self.__dict__ and "norms" not in self._modules:
+            self.norms = None  # pickled before models could hold norms
+
     def _hidden(self, data, layout: Optional[GraphLayout] = None) -> torch.Tensor:
         x, edge_index, edge_attr = data.x, data.edge_index, data.edge_attr
         if self.standardize:

@@ -32,3 +32,21 @@ def test_unknown_optimizer_in_the_loop():
     assert not model.training
     assert all(p.grad is None for p in model.parameters())
     assert isinstance(model.gat_layers[0].lin_src.weight, torch.nn.Parameter)
+
+
+def test_model_pickled_without_norms():
+    """A whole model pickled before it could hold norms is a model without them."""
+    import copy
+    import io
+    model = _model()
+    old = copy.deepcopy(model)
+    del old.__dict__["norms"]
+    buf = io.BytesIO()
+    torch.save(old, buf)
+    buf.seek(0)
+    again = torch.load(buf, weights_only=False)  # (this test's own bytes)
+    assert again.norms is None
+    assert copy.deepcopy(again).norms is None
+    from spotv2net_amd import GATModel
+    normed = GATModel(60, 6, 2, 1, [8, 4], concat_heads=True, layer_norm=True)
+    assert len(copy.deepcopy(normed).norms) == 2
