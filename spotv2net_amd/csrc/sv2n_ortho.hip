@@ -39,8 +39,10 @@
 // product's fragments straight from registers.
 //
 // Several matrices (a model's weights) share each launch: `first` maps blocks to
-// matrices, so a step over four weights costs the same 3·steps + 2 launches as one.
-// Small and thin matrices take fewer (k_ns_qx, k_ns_thin).
+// matrices, so four weights cost as many launches as one: two, and three to six a step
+// (a product whose last tiles of 128 fill no round takes a second one, ns_product).
+// Small and thin matrices take fewer (k_ns_qx, k_ns_thin), thin ones beside large ones
+// add one and one a step.
 #include "sv2n_common.h"
 #include <algorithm>
 #include <cmath>
@@ -55,10 +57,26 @@ constexpr int NS_PARTS = 1024;  // most partial sums of squares of one matrix
 constexpr int NS_PART_ELEMS = 4096;
 constexpr int NS_THIN_COLS = 128;  // columns of a thin matrix a block keeps
 constexpr int NS_EXACT = 32;    // smaller sides up to which the products are always f32
-constexpr int NS_THIN_LONG = 2048;  // length from which a thin matrix has launches of its own
-constexpr int NS_HALF = 128;    // tiles of 128 that are worth a round of their own
-constexpr int NS_FUSED = 512;   // tiles of 32 up to which blocks make their own rows of Q
-constexpr int NS_TINY = 72;     // tiles of 64 below which tiles of 32 are faster
+// The bounds between variants; us of the whole five steps, in a captured graph.
+// Length from which thin matrices beside small ones get launches of their own.  16 x n
+// beside 128 x 128, riding along / own: n 1,024 94 / 104, 1,408 103 / 107, 1,536 110 / 105,
+// 4,096 196 / 117 (beside six of 64 x 64, or 400 x 300 and 200 x 400, the same n).
+constexpr int NS_THIN_LONG = 1408;
+// Tiles of 128 that are worth a round of their own (else they are cut into tiles of 64).
+// n² at 64 / 128 / 256: 1,300 (121 tiles) 471 / 265 / 263, 2,300 (324, 68 left over)
+// 996 / 975 / 1,069, 2,700 (484, 228 left over) 1,308 / 1,305 / 1,752.
+constexpr int NS_HALF = 128;
+// Tiles of 32 of X up to which blocks make their own rows of Q.  128 x n, own / a launch
+// for Q: 16 tiles 69 / 73, 256 97 / 101, 512 134 / 133, 752 172 / 166, 2,048 373 / 321.
+constexpr int NS_FUSED = 512;
+// Tiles of 64 of a product below which tiles of 32 are faster, 32 / 64: 400 x 400 (28 of
+// S, 49 of X) 91 / 116, 704² (66, 121) 137 / 155, 768² (78, 144) 174 / 158, 1,024² (136,
+// 256) 265 / 184.
+constexpr int NS_TINY = 72;
+// Depth of X's product from which tiles of 128 are worth it, 128 / 64: 1,024 x 2,048
+// 291 / 252, 1,152 x 2,048 309 / 304, 1,260 x 3,000 394 / 406, 1,792² 545 / 604, 2,048 x
+// 8,192 1,974 / 2,409.
+constexpr int NS_DEEP = 1200;
 
 struct NsMat {
   const void* g;        // [batch][rows][ld] of dtype
@@ -657,7 +675,7 @@ __global__ __launch_bounds__(64 * W, FT == 4 ? 1 : 2) void k_ns_mm(NsArgs A, NsS
 // ---- 3b: Q and X's product in one launch, for small matrices (mp <= 128) ----
 // A 32 x 32 tile of X needs 32 rows of Q, 32 x m values from the m x m S: each block
 // makes them itself (in LDS, as fragments) rather than wait for a launch that stores
-// Q.  128 x 1,024: 4.3 + 4.5 us in two launches, 7.9 in one (92 -> 81 us with all steps).
+// Q.  128 x 1,024: 4.3 + 4.5 us in two launches, 7.9 in one (87 -> 81 us with all steps).
 // Eight waves: first Q's m / 32 tiles times
 // slices of their depth, then 16 K values of X's product each.
 template <int EPI>
@@ -1014,12 +1032,11 @@ static void ns_shape(NsMat* M) {
 }
 
 // What a group's matrices are padded to: 128 where X's product (the largest) is worth
-// tiles of 128: enough of them, and at least 1,024 deep (K 777, 273 tiles: 47.4 us
-// against 31.8 on tiles of 64), else 64
+// tiles of 128: NS_HALF of them that are NS_DEEP deep, else 64
 static int ns_pad(const NsMat* mats, int count) {
   int64_t tiles = 0;
   for (int i = 0; i < count; ++i)
-    if (mats[i].m >= 1024)
+    if (mats[i].m >= NS_DEEP)
       tiles += (int64_t)mats[i].batch * (ns_up(mats[i].m, 128) / 128) *
                (ns_up(mats[i].n, 128) / 128);
   return tiles >= NS_HALF ? 128 : 64;

@@ -83,9 +83,10 @@ def muon_step(weights: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
 class Muon(torch.optim.Optimizer):
     """Momentum with orthogonalised updates for weight matrices (2-D float32
     parameters); everything else belongs to another optimiser.  One ``step`` is
-    at most ``3 steps + 2`` launches per 16 matrices of a parameter group (a few more
-    where thin ones stand beside large ones), without a host synchronisation, and can
-    be captured into a graph after a first step outside of it."""
+    ``2 + 3 steps`` launches per 16 matrices of a parameter group (sides past about
+    1,200: up to twice as many; thin matrices beside large ones: ``1 + steps`` more;
+    small ones alone: fewer), without a host synchronisation, and can be captured into
+    a graph after a first step outside of it."""
 
     def __init__(self, params, lr: float = 1e-3, weight_decay: float = 0.1, momentum: float = 0.95,
                  nesterov: bool = True, coefficients: Tuple[float, float, float] = COEFFICIENTS,
