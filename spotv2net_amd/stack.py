@@ -167,7 +167,12 @@ class _GradTargets:
     def returned(self) -> tuple:
         if self.direct:
             return (None,) * len(self._order)
-        return tuple(self._views.get(i) if i in self._used else None for i in self._order)
+        # a parameter that occurs twice has both uses in its one buffer
+        given, out = set(), []
+        for i in self._order:
+            out.append(self._views.get(i) if i in self._used and i not in given else None)
+            given.add(i)
+        return tuple(out)
 
 
 def _stand_in(params, device) -> torch.Tensor:
@@ -592,6 +597,9 @@ def stack_backward(saved, meta: _StackMeta, convs, layout: GraphLayout, dout, ne
     dev = dout.device
     B, n, N = layout.num_graphs, layout.n, layout.num_nodes
 
+    # layers that share a parameter add to one buffer: one after the other
+    ids = [id(p) for c in convs for p in layer_params(c)]
+    tied = len(set(ids)) < len(ids)
     dy = dout.contiguous()
     daes = [None] * L
     dwf = torch.zeros_like(wf) if fused else None  # every layer writes its own columns
@@ -621,7 +629,7 @@ def stack_backward(saved, meta: _StackMeta, convs, layout: GraphLayout, dout, ne
             elif not fused and not edge_tail:
                 dwf = ops.edge_logits_bwd(ea, ei, layout.canon, daes, H, B, n, hp,
                                           layout.tiled)
-            if all(a is not None and b is not None for a, b in need_e):
+            if not tied and all(a is not None and b is not None for a, b in need_e):
                 # every layer's edge-fold backward in one launch
                 ops.prep_bwd_edge_all(dwf, [l * H for l in range(L)],
                                       [c.lin_edge.weight for c in convs],
@@ -640,7 +648,7 @@ def stack_backward(saved, meta: _StackMeta, convs, layout: GraphLayout, dout, ne
     # hand their memory to a main-stream allocation while the side stream
     # still reads them), and the gradient buffers it writes are only read
     # after the join
-    side = _side_stream(dev) if _overlap_bwd(dev, meta.bf16) else None
+    side = _side_stream(dev) if _overlap_bwd(dev, meta.bf16) and not tied else None
     main = torch.cuda.current_stream(dev) if side is not None else None
     held = []
     edge_forked = False
