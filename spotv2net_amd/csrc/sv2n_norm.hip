@@ -9,7 +9,8 @@
 // deviations from it (added to the mean), then the squares of those left costs no second
 // read and loses nothing to cancellation: a row of equal values has exactly that mean,
 // z = 0 and variance 0, where a mean off by its rounding would come out scaled by rstd,
-// up to 1/sqrt(eps).  TPR is the smallest group that leaves a thread at most 16 elements
+// up to 1/sqrt(eps).  (The factors 1/cols are rounded too: the first is corrected, the
+// second moves a correction of a few units by far less than one.)  TPR is the smallest group that leaves a thread at most 16 elements
 // (32 past rows of 8,192), since the backward holds five such arrays (x, dy, w and the
 // sums of dw and db): 16 threads for a row of 128, so a wave carries four of them.
 // Groups walk the rows with a stride; each thread owns the same columns in every
@@ -27,9 +28,14 @@
 // instead of branching; a group past the last row adds zeros.
 //
 // MI355X, us (forward / backward with its second launch; a large copy reaches 5.0 TB/s):
-//   15,360 x 400 f32      11.3 / 18.7        16,384 x 4,096 f32    91 / 163  (5.9 / 5.1 TB/s)
-//   262,144 x 128 f32       45 / 82          16,384 x 8,192 bf16   97 / 160  (5.6 / 5.2 TB/s)
-//   3,840 x 3,000 bf16    12.6 / 28.3        10,007 x 1,261 f16  17.4 / 26.7
+//   15,360 x 400 f32      10.5 / 18.5        16,384 x 4,096 f32    97 / 158  (5.5 / 5.1 TB/s)
+//   262,144 x 128 f32       45 / 81          16,384 x 8,192 bf16  100 / 153  (5.4 / 5.3 TB/s)
+//   3,840 x 3,000 bf16    12.0 / 27.8        10,007 x 1,261 f16  18.2 / 25.9
+// The last two are 1.3 and 1.8 (forward), 2.0 and 1.7 (backward) times a copy of their
+// bytes: rows of 375 and 158 vectors leave a quarter and three eighths of the places for
+// vectors empty, the backward's partials are a quarter and a fifth of its bytes again
+// (written and read, 17 and 15 MB), and 360 blocks for 3,840 rows give 104 of the 256 CUs
+// 22 rows and the others 11.
 #include "sv2n_common.h"
 #include <algorithm>
 #include <type_traits>
@@ -207,6 +213,15 @@ __global__ __launch_bounds__(ln_threads<TPR>()) void k_ln_fwd(
     ln_ld_w<T>(b, wdt, at[k], 0.f, bv[k]);
   }
   const float inv_c = 1.f / (float)cols;
+  // (rows of several waves: of the elements of this wave, if any)
+  float inv_n = inv_c;
+  if constexpr (WPR > 1) {
+    int n = 0;
+#pragma unroll
+    for (int k = 0; k < NPT; ++k)
+      n += max(0, min(64 * V, cols - k * TPR * V - (t / 64) * 64 * V));
+    inv_n = 1.f / (float)max(n, 1);
+  }
   const int64_t step = (int64_t)gridDim.x * GROUPS;
   LnRaw<T> next[NPT];
   auto fetch = [&](int64_t row) {
@@ -219,6 +234,9 @@ __global__ __launch_bounds__(ln_threads<TPR>()) void k_ln_fwd(
   // the block's first row decides how often it goes round: its groups stay together
   int buf = 0;
   for (int64_t r0 = (int64_t)blockIdx.x * GROUPS; r0 < rows; r0 += step, row += step) {
+    // (a deviation is from the rounded mean that the correction is added to, not from an
+    // unrounded product inside a fused operation)
+#pragma clang fp contract(off)
     float v[NPT][V];
     float s = 0.f;
 #pragma unroll
@@ -230,21 +248,12 @@ __global__ __launch_bounds__(ln_threads<TPR>()) void k_ln_fwd(
       }
     fetch(row + step);
     s = group_sum<G>(s);
-    float m, m1 = 0.f, m2 = 0.f;
-    int n = cols;  // elements of the group, or (rows of several waves) of the wave
-    if constexpr (WPR > 1) {
-      const int wv0 = (t / 64) * 64 * V;
-      n = 0;
-#pragma unroll
-      for (int k = 0; k < NPT; ++k) n += max(0, min(64 * V, cols - k * TPR * V - wv0));
-    }
-    const float fn = (float)max(n, 1);
-    m = s / fn;
+    float m = s * inv_n, m1 = 0.f, m2 = 0.f;
 #pragma unroll
     for (int k = 0; k < NPT; ++k)
 #pragma unroll
       for (int j = 0; j < V; ++j) m1 += k < NPT - 1 || at[k].has(j) ? v[k][j] - m : 0.f;
-    m += group_sum<G>(m1) / fn;
+    m += group_sum<G>(m1) * inv_n;
 #pragma unroll
     for (int k = 0; k < NPT; ++k)
 #pragma unroll
@@ -271,7 +280,7 @@ __global__ __launch_bounds__(ln_threads<TPR>()) void k_ln_fwd(
         for (int k = 0; k < NPT; ++k) n += max(0, min(64 * V, cols - k * TPR * V - u * 64 * V));
         tot = fmaf((float)n, mine[u][0] - m0, tot);
       }
-      m = m0 + tot / (float)cols;
+      m = fmaf(tot, inv_c, m0);
 #pragma unroll
       for (int u = 0; u < WPR; ++u) {
         int n = 0;
