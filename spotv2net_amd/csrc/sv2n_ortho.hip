@@ -1209,7 +1209,8 @@ static void ns_run_as(NsArgs& A, const NsScale& sc, int steps, int pad, hipStrea
 // (a step's launches are shared), else those of m <= NS_EXACT have them alone
 static void ns_exact(NsArgs* A, const NsRange& range) {
   bool all = false;
-  for (int i = 0; i < A->count; ++i) all |= !ns_pairs_ok(A->mat[i], range);
+  for (int i = 0; i < A->count; ++i)
+    all |= A->mat[i].m > NS_EXACT && !ns_pairs_ok(A->mat[i], range);
   for (int i = 0; i < A->count; ++i) A->mat[i].exact = all || A->mat[i].m <= NS_EXACT;
 }
 

@@ -108,3 +108,16 @@ def test_optimizer_step(dev, shapes):
         ref = definition(g, steps=16) * -math.sqrt(max(1.0, g.shape[0] / g.shape[1]))
         f32 = rel(definition(g, steps=16, dtype=torch.float32), definition(g, steps=16))
         assert rel(w, ref) <= max(3 * f32, 3e-5), tuple(g.shape)
+
+
+def test_long_thin_neighbour(dev):
+    """A thin matrix is on f32 products anyway: beside it the others keep theirs (the
+    bits of the step without it)."""
+    from spotv2net_amd import muon_step
+    g, t = graded(dev, 96, 128, 1.0, "rows")[0], graded(dev, 30, 16384, 1.0, "rows", seed=1)[0]
+    both, alone = [torch.zeros_like(g), torch.zeros_like(t)], [torch.zeros_like(g)]
+    for steps in (8, 16):
+        muon_step(both, [g, t], [torch.zeros_like(g), torch.zeros_like(t)], lr=1.0, momentum=0.0,
+                  steps=steps)
+        muon_step(alone, [g], [torch.zeros_like(g)], lr=1.0, momentum=0.0, steps=steps)
+        assert torch.equal(both[0], alone[0]), steps
