@@ -26,6 +26,22 @@ def tie(model, what):
     return model
 
 
+def test_replayed_graphs(dev):
+    """Layers used twice in the plain loop: its replayed graphs against eager runs."""
+    from spotv2net_amd import GATModel, synthetic_batch
+    torch.manual_seed(0)
+    model = GATModel(60, 6, 4, 1, [8, 8, 8, 8], concat_heads=True).to(dev).train()
+    model.gat_layers[2] = model.gat_layers[1]
+    data = synthetic_batch(3, 2, seed=5, device=dev)
+    model.graph_replay = False
+    want = torch.autograd.grad(model(data).sum(), list(model.parameters()))
+    model.graph_replay = True
+    for _ in range(5):
+        got = torch.autograd.grad(model(data).sum(), list(model.parameters()))
+        for (k, _), a, b in zip(model.named_parameters(), got, want):
+            assert_close(a, b, tol=1e-5, what=k)
+
+
 @pytest.mark.parametrize("what", ["norms", "norm weights", "layers", "layer weights"])
 @pytest.mark.parametrize("direct", [False, True])
 @pytest.mark.parametrize("n", [30, 40])
