@@ -744,7 +744,8 @@ int sv2n_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx
  * bits: where the smaller side is above 32 and the steps could not make it visible
  * (the default coefficients: up to five steps at every size, six to 4,096 x 4,096,
  * eight to 64 x 128), X is held to 2^-39 of max(|G|_F, eps) and 22 bits of an entry,
- * so rows or columns under 2^-16 of it lose bits and under 2^-39 are taken as 0.
+ * so rows or columns under 2^-16 of it lose bits and under 2^-39 are taken as 0
+ * (and all of a matrix whose norm is that far below eps).
  * Other calls use f32 products throughout (1.1 to 4 times the time).
  * Sides up to SV2N_NS_MAX_SIDE, steps 1..SV2N_NS_MAX_STEPS, batch up to
  * SV2N_NS_MAX_BATCH.  Coefficients that let a singular value grow past 256 are
