@@ -60,10 +60,10 @@ constexpr int NS_EXACT = 32;    // smaller sides up to which the products are al
 // The bounds between variants; us of the whole five steps, in a captured graph.
 // Length from which thin matrices beside small ones get launches of their own.  16 x n
 // beside 128 x 128, riding along / own: n 1,024 94 / 104, 1,408 103 / 107, 1,536 110 / 105,
-// 4,096 196 / 117 (beside six of 64 x 64, or 400 x 300 and 200 x 400, the same n).
+// 4,096 196 / 117 (beside six of 64 x 64, or 400 x 300 and 200 x 400, they cross there too).
 constexpr int NS_THIN_LONG = 1408;
 // Tiles of 128 that are worth a round of their own (else they are cut into tiles of 64).
-// n² at 64 / 128 / 256: 1,300 (121 tiles) 471 / 265 / 263, 2,300 (324, 68 left over)
+// n² at 48 / 128 / 256: 1,300 (121 tiles) 471 / 265 / 263, 2,300 (324, 68 left over)
 // 996 / 975 / 1,069, 2,700 (484, 228 left over) 1,308 / 1,305 / 1,752.
 constexpr int NS_HALF = 128;
 // Tiles of 32 of X up to which blocks make their own rows of Q.  128 x n, own / a launch
